@@ -22,7 +22,9 @@ OBJ = os.path.join(CSRC, ".build")
 OUT = os.path.join(CSRC, "libvitta_hip.so")
 KEYFILE = OUT + ".sha256"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + os.environ.get("VITTA_EXTRA_CFLAGS", "").split()  # (experiments)
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results now and then on this card
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED_F32 + os.environ.get("VITTA_EXTRA_CFLAGS", "").split()  # (experiments)
 LDFLAGS = ["--offload-arch=gfx950", "-shared", "-fPIC"]
 JOBS = int(os.environ.get("VITTA_BUILD_JOBS", "6"))
 
