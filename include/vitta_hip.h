@@ -870,6 +870,52 @@ int vitta_frames_cv2_resize(const uint8_t* d_frames, int32_t n_frames, int32_t i
                             int32_t mode, const int32_t* d_tables, int32_t out_h, int32_t out_w, uint8_t* d_out_u8,
                             float* d_out_f32, int32_t clip_len, const float* d_mean, const float* d_stdinv, void* stream);
 
+/* --------------------------------------------------------------------------
+ * Rows of class scores (logits): what they say of a label, how sure they are, and a loss against another model's answer.
+ *   d_x     [rows][row_stride] scores, classes of them used per row (row_stride in elements, any >= 0); dtype one of the
+ *           VITTA_SCORES_* below, element aligned;  z = x / temperature,  p = softmax(z)
+ * vitta_label_logprobs_fwd, any of the outputs may be NULL:
+ *   d_logprob [rows]      z_y - lse of label y = d_labels[row]; 0 where y == ignore_index, NaN where y is no class (nothing is read)
+ *   d_entropy [rows]      -sum p log p        d_lse [rows]  log sum exp z
+ *   d_top_logprob, d_top_index [rows][top]    the `top` highest scores in falling order, ties to the lowest class; index -1 (and log
+ *                         probability -inf) where fewer classes have a score above -inf.  top <= VITTA_SCORES_MAX_TOP, <= classes
+ *   d_stats [rows][4]     row statistics for the backward (16-byte aligned)
+ *   A row of -inf only: log probabilities -inf, entropy 0, gradient 0.  A row with a NaN or +inf: NaN everywhere, indices -1.
+ * vitta_label_logprobs_bwd: d_dx [rows][classes] (dtype, dense) from the upstream gradients, each NULL or a float per row at the given
+ *   element stride (0: one value for every row); d_gtop [rows][top] dense.  A row whose upstream gradients are all 0 gets zeros.
+ * vitta_top_distill_fwd: d_loss[row] = KL(teacher's list || student)
+ *   d_index, d_value [rows][list]  the teacher's classes and scores; an index that is no class (-1) is padding; a row of padding only
+ *           has loss 0 and gradient 0.  A class listed twice counts with the sum of its probabilities.
+ *   tail == 0: q = softmax(d_value / temperature) over the list
+ *   tail != 0: d_value are log probabilities; what they leave of 1 belongs to the classes outside the list as one class (left out
+ *           where the student gives these nothing)
+ *   d_q [rows][list], d_stats [rows][4]  for the backward.    list <= VITTA_SCORES_MAX_LIST
+ * vitta_top_distill_bwd: d_dx [rows][classes] from d_g, a float per row at stride g_stride.
+ * Workspace: vitta_scores_workspace_bytes(rows, classes, dtype, top) (top = 0 for the distillation), 256-byte aligned, may be 0;
+ * one call's own until its launches have run.
+ * -------------------------------------------------------------------------- */
+#define VITTA_SCORES_F32 0
+#define VITTA_SCORES_BF16 1
+#define VITTA_SCORES_F16 2
+#define VITTA_SCORES_MAX_TOP 64
+#define VITTA_SCORES_MAX_LIST 256
+size_t vitta_scores_workspace_bytes(int64_t rows, int32_t classes, int32_t dtype, int32_t top);
+int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+                             const int64_t* d_labels, int64_t ignore_index, int32_t top, float* d_logprob, float* d_entropy,
+                             float* d_lse, float* d_top_logprob, int64_t* d_top_index, float* d_stats, void* d_workspace,
+                             size_t workspace_bytes, void* stream);
+int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+                             const int64_t* d_labels, int64_t ignore_index, int32_t top, const int64_t* d_top_index,
+                             const float* d_stats, const float* d_glogprob, int64_t glogprob_stride, const float* d_gentropy,
+                             int64_t gentropy_stride, const float* d_glse, int64_t glse_stride, const float* d_gtop, void* d_dx,
+                             void* stream);
+int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+                          const int64_t* d_index, const void* d_value, int32_t value_dtype, int32_t list, int32_t tail, float* d_loss,
+                          float* d_stats, float* d_q, void* d_workspace, size_t workspace_bytes, void* stream);
+int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+                          const int64_t* d_index, int32_t list, const float* d_stats, const float* d_q, const float* d_g,
+                          int64_t g_stride, void* d_dx, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,7 @@ class LayerShape(C.Structure):
     _fields_ = [("outer", C.c_int64), ("C", C.c_int32), ("inner", C.c_int64), ("layout", C.c_int32)]
 
 
+SCORES_MAX_TOP, SCORES_MAX_LIST = 64, 256
 CONV_MAX_TAPS = 9
 
 
@@ -99,6 +100,12 @@ SIGNATURES = {
     "vitta_stat_align_fwd_f32": (C.c_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _f32, C.c_int,
                                            _p, _p, _p, _p, _p, _p, _p]),
     "vitta_stat_align_bwd_f32": (C.c_int, [_p, _p, _p, _i64, _i32, _i64, _i32, _p, _p, _p, _p, _p]),
+    "vitta_scores_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "vitta_label_logprobs_fwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _f32, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "vitta_label_logprobs_bwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _f32, _p, _i64, _i32, _p, _p, _p, _i64, _p, _i64, _p, _i64,
+                                           _p, _p, _p]),
+    "vitta_top_distill_fwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _f32, _p, _p, _i32, _i32, _i32, _p, _p, _p, _p, _sz, _p]),
+    "vitta_top_distill_bwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _f32, _p, _i32, _p, _p, _p, _i64, _p, _p]),
     "vitta_pred_consis_f32": (C.c_int, [_p, _i32, _i32, _i32, _p, _p, _p]),
     "vitta_tam_pool_f32": (C.c_int, [_p, _i32, _i32, _i32, _i32, _p, _p]),
     "vitta_tam_agg_fwd_f32": (C.c_int, [_p, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),

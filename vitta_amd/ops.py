@@ -6,8 +6,10 @@ is no eager fallback for the HIP path.
 """
 import ctypes as C
 import os
+from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import LAYOUT_NCHW, LAYOUT_NHWC, REG_TYPES, check, lib
@@ -143,6 +145,194 @@ class PredConsis(torch.autograd.Function):
 
 def pred_consis(preds):
     return PredConsis.apply(preds)
+
+
+# ------------------------------------------------------------------------------------------------
+# rows of class scores: log probabilities, entropy, best alternatives; distillation from a teacher's top list
+# ------------------------------------------------------------------------------------------------
+_SCORE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class LabelLogprobs(NamedTuple):
+    """What `label_logprobs` answers; None for what was not asked."""
+    logprob: Optional[torch.Tensor]
+    entropy: Optional[torch.Tensor]
+    lse: torch.Tensor
+    top_logprob: Optional[torch.Tensor]
+    top_index: Optional[torch.Tensor]
+
+
+def _score_rows(x, name, temperature):
+    """(rows of the scores as a matrix whose last stride is 1, leading shape, classes, row stride); copies only what has no such view."""
+    if not x.is_cuda:
+        raise _lib.VittaHipError(f"{name} must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
+    if x.dtype not in _SCORE_TYPES:
+        raise _lib.VittaHipError(f"{name} must be float32, bfloat16 or float16 (got {x.dtype})")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{name} must hold classes in its last dimension (got shape {tuple(x.shape)})")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature must be a positive finite number (got {temperature})")
+    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if m.stride(1) != 1 or m.stride(0) < 0:
+        m = m.contiguous()
+    return m, x.shape[:-1], m.shape[1], m.stride(0)
+
+
+def _score_side(t, name, like, shape, dtypes):
+    """A companion of the scores (labels, a teacher's list): on their device, of the given shape and one of the types, dense."""
+    if t.device != like.device:
+        raise _lib.VittaHipError(f"{name} must live on {like.device} like the scores (got {t.device})")
+    if t.dtype not in dtypes:
+        raise _lib.VittaHipError(f"{name} must be one of {[str(d) for d in dtypes]} (got {t.dtype})")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
+    return (t.long() if t.dtype == torch.int32 else t).contiguous()
+
+
+def _score_workspace(m, rows, classes, top):
+    n = int(lib().vitta_scores_workspace_bytes(rows, classes, _SCORE_TYPES[m.dtype], top))
+    return (torch.empty(n, dtype=torch.uint8, device=m.device) if n else None), n
+
+
+def _row_gradient(g, rows):
+    """(tensor or None, stride) of an upstream gradient per row; one value for every row (what mean() and sum() send) is not spread out."""
+    if g is None:
+        return None, 0
+    if rows > 1 and all(s == 0 or n == 1 for s, n in zip(g.stride(), g.shape)):
+        return g, 0
+    return g.contiguous(), 1
+
+
+def _label_logprobs(m, lead, labels, top, entropy, temperature, ignore_index, stats):
+    rows, classes = m.shape
+    f = dict(dtype=torch.float32, device=m.device)
+    logprob = torch.empty(lead, **f) if labels is not None else None
+    ent = torch.empty(lead, **f) if entropy else None
+    lse = torch.empty(lead, **f)
+    top_logprob = torch.empty(*lead, top, **f) if top else None
+    top_index = torch.empty(*lead, top, dtype=torch.int64, device=m.device) if top else None
+    if rows:
+        with torch.cuda.device(m.device):
+            ws, n = _score_workspace(m, rows, classes, top)
+            check(lib().vitta_label_logprobs_fwd(_p(m), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _p(labels),
+                                                 ignore_index, top, _p(logprob), _p(ent), _p(lse), _p(top_logprob), _p(top_index),
+                                                 _p(stats), _p(ws), n, _stream()), "vitta_label_logprobs_fwd")
+    return logprob, ent, lse, top_logprob, top_index
+
+
+class _LabelLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, labels, top, entropy, temperature, ignore_index):
+        m, lead, _, _ = _score_rows(x, "logits", temperature)
+        stats = torch.empty(m.shape[0], 4, dtype=torch.float32, device=m.device)
+        out = _label_logprobs(m, lead, labels, top, entropy, temperature, ignore_index, stats)
+        ctx.save_for_backward(m, labels, out[4], stats)
+        ctx.how = (x.shape, top, temperature, ignore_index)
+        if top:
+            ctx.mark_non_differentiable(out[4])
+        ctx.set_materialize_grads(False)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logprob, g_entropy, g_lse, g_top, _):
+        m, labels, top_index, stats = ctx.saved_tensors
+        shape, top, temperature, ignore_index = ctx.how
+        rows, classes = m.shape
+        dx = torch.empty(shape, dtype=m.dtype, device=m.device)
+        if rows:
+            (a, sa), (b, sb), (c, sc) = _row_gradient(g_logprob, rows), _row_gradient(g_entropy, rows), _row_gradient(g_lse, rows)
+            g_top = g_top.contiguous() if g_top is not None else None
+            with torch.cuda.device(m.device):
+                check(lib().vitta_label_logprobs_bwd(_p(m), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _p(labels),
+                                                     ignore_index, top, _p(top_index), _p(stats), _p(a), sa, _p(b), sb, _p(c), sc,
+                                                     _p(g_top), _p(dx), _stream()), "vitta_label_logprobs_bwd")
+        return dx, None, None, None, None, None
+
+
+def label_logprobs(logits, labels=None, *, top=0, entropy=True, temperature=1.0, ignore_index=-100):
+    """Log probability of given labels, entropy and best alternatives of rows of class scores, read once.
+
+    logits (..., V) float32 / bfloat16 / float16 (rows may be cut from a wider matrix); labels (...) int64 or int32, or None.
+    Returns a LabelLogprobs of float32 tensors shaped (...): with z = logits / temperature,
+      logprob       z[label] - lse; 0 where label == ignore_index; NaN where the label is no class
+      entropy       -sum p log p, p = softmax(z) (None with entropy=False)
+      lse           log sum exp z
+      top_logprob, top_index (..., top): the `top` (at most 64) best classes in falling order, ties to the lowest index; index -1 and
+                    log probability -inf where fewer classes have a score above -inf.
+    A row of -inf only has log probabilities -inf, entropy 0 and gradient 0; a row with NaN or +inf answers NaN and -1.
+    Differentiable once in logits through logprob, entropy, lse and top_logprob; the gradient has the logits' type."""
+    _score_rows(logits, "logits", temperature)
+    if not 0 <= top <= min(_lib.SCORES_MAX_TOP, logits.shape[-1]):
+        raise ValueError(f"top must be between 0 and min({_lib.SCORES_MAX_TOP}, classes = {logits.shape[-1]}) (got {top})")
+    if labels is not None:
+        labels = _score_side(labels, "labels", logits, logits.shape[:-1], (torch.int64, torch.int32))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return LabelLogprobs(*_LabelLogprobs.apply(logits, labels, int(top), bool(entropy), float(temperature), int(ignore_index)))
+    m, lead, _, _ = _score_rows(logits, "logits", temperature)
+    return LabelLogprobs(*_label_logprobs(m, lead, labels, int(top), entropy, float(temperature), int(ignore_index), None))
+
+
+def _top_distill(m, lead, index, value, temperature, tail):
+    rows, classes = m.shape
+    f = dict(dtype=torch.float32, device=m.device)
+    loss, stats, q = torch.empty(lead, **f), torch.empty(rows, 4, **f), torch.empty(index.shape, **f)
+    if rows:
+        with torch.cuda.device(m.device):
+            ws, n = _score_workspace(m, rows, classes, 0)
+            check(lib().vitta_top_distill_fwd(_p(m), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _p(index), _p(value),
+                                              _SCORE_TYPES[value.dtype], index.shape[-1], int(tail), _p(loss), _p(stats), _p(q), _p(ws), n,
+                                              _stream()), "vitta_top_distill_fwd")
+    return loss, stats, q
+
+
+class _TopDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, index, value, temperature, tail):
+        m, lead, _, _ = _score_rows(x, "student_logits", temperature)
+        loss, stats, q = _top_distill(m, lead, index, value, temperature, tail)
+        ctx.save_for_backward(m, index, stats, q)
+        ctx.how = (x.shape, temperature)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        m, index, stats, q = ctx.saved_tensors
+        shape, temperature = ctx.how
+        rows, classes = m.shape
+        dx = torch.empty(shape, dtype=m.dtype, device=m.device)
+        if rows:
+            g, sg = _row_gradient(g, rows)
+            with torch.cuda.device(m.device):
+                check(lib().vitta_top_distill_bwd(_p(m), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _p(index),
+                                                  index.shape[-1], _p(stats), _p(q), _p(g), sg, _p(dx), _stream()), "vitta_top_distill_bwd")
+        return dx, None, None, None, None
+
+
+def top_distill(student_logits, teacher_index, teacher_value, *, temperature=1.0, tail=False):
+    """KL divergence of a student from a teacher of whom only a list of best classes is kept, a float32 loss per row.
+
+    student_logits (..., V) float32 / bfloat16 / float16; teacher_index (..., K) int64 or int32 and teacher_value (..., K) float32 /
+    bfloat16 / float16, K at most 256, without gradient; an index that is no class (-1, as `label_logprobs` gives) is padding, and a
+    row of padding only has loss 0 and gradient 0.  p = softmax(student_logits / temperature) over all V classes, and
+      tail=False  q = softmax(teacher_value / temperature) over the list:  sum q (log q - log p)
+      tail=True   teacher_value are log probabilities (at the same temperature); what they leave of 1 is one more class against what the
+                  student gives the classes outside the list (left out where that is nothing).
+    A class listed twice counts with the sum of its probabilities.  No factor temperature ** 2 is applied.  Differentiable once in
+    student_logits; the gradient has their type."""
+    _score_rows(student_logits, "student_logits", temperature)
+    if teacher_index.dim() == 0 or not 1 <= teacher_index.shape[-1] <= _lib.SCORES_MAX_LIST:
+        raise ValueError(f"teacher_index must hold 1 to {_lib.SCORES_MAX_LIST} classes per row (got shape {tuple(teacher_index.shape)})")
+    if teacher_value.requires_grad:
+        raise ValueError("teacher_value gets no gradient: detach it")
+    shape = student_logits.shape[:-1] + teacher_index.shape[-1:]
+    index = _score_side(teacher_index, "teacher_index", student_logits, shape, (torch.int64, torch.int32))
+    value = _score_side(teacher_value, "teacher_value", student_logits, shape, tuple(_SCORE_TYPES))
+    if torch.is_grad_enabled() and student_logits.requires_grad:
+        return _TopDistill.apply(student_logits, index, value, float(temperature), bool(tail))
+    m, lead, _, _ = _score_rows(student_logits, "student_logits", temperature)
+    return _top_distill(m, lead, index, value, float(temperature), tail)[0]
 
 
 # ------------------------------------------------------------------------------------------------
