@@ -2,10 +2,19 @@
 // teacher's top list (vitta_top_distill_*), forward and gradient.
 //
 // With x the scores of a row, T the temperature, c = log2(e) / T, m = max x, a_j = (x_j - m) c, e_j = 2^a_j, s = sum e, t = sum e a:
-//   log p_j = ln2 (a_j - log2 s)        entropy = ln2 (log2 s - t / s)        lse = m / T + ln2 log2 s
+//   log p_j = (x_j - m) / T - ln2 log2 s        entropy = ln2 (log2 s - t / s)        lse = m / T + ln2 log2 s
 // The difference x - m is taken first, so the best score's term is exactly 1 and a row of the type's lowest value stays finite.
 // m starts at the lowest finite float: a row of minus infinities keeps s = 0 and is answered as a row without a distribution.
 // Sums, maxima and statistics are 32 bits wide; a gradient is rounded once, to the scores' type.
+//
+// Forward: one pass.  A lane holds four 16-byte loads while the next four are on their way, takes their maximum, moves its running sums to
+// it and adds; the lanes' (m, s, t) are joined at the end.  A short row (<= kWaveRow classes) belongs to one wave, a longer one to a
+// workgroup of eight, and few long rows are cut into segments whose results a second launch joins.
+// Best alternatives in the same pass: a lower bound of the k-th best (from the lanes' maxima of the first loads) lets all but a few scores
+// pass by; the few go to a buffer of their wave in LDS, and every 64 of them are sorted across the lanes and merged into the wave's
+// list of 64.  Equal scores order by class, so the answer does not depend on which wave saw what.
+// Gradient: elementwise from the row statistics, e_j (A + B a_j); the few classes that a label or a list adds to are written again at the end
+// by the workgroup that wrote them.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -18,7 +27,55 @@ using namespace vitta;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLowest = -3.402823466e+38f;
-constexpr int kThreads = 256;
+constexpr int kU = 4;              // 16-byte loads of a lane that are consumed together
+constexpr int kWaves = 8;          // waves of a workgroup that share a long row
+constexpr int kWaveRow = 4096;     // classes up to which a row belongs to one wave
+constexpr int kBuf = 64 + 8 * 64;  // candidates of a wave: 63 waiting and a whole vector of every lane
+constexpr int kMaxSegments = 64;
+constexpr int kTailSegment = 1 << 18;  // classes whose membership bits fit 32 KiB
+
+// ---- element types -------------------------------------------------------------------------------------------------------------
+template <typename T> struct Pack;
+template <> struct Pack<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ uint4 empty() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  static __device__ __forceinline__ void open(const uint4& w, float* f) {
+    f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ uint4 close(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <> struct Pack<__hip_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ uint4 empty() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  static __device__ __forceinline__ void open(const uint4& w, float* f) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint32_t two(float a, float b) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, bf2));
+  }
+  static __device__ __forceinline__ uint4 close(const float* f) { return make_uint4(two(f[0], f[1]), two(f[2], f[3]), two(f[4], f[5]), two(f[6], f[7])); }
+};
+template <> struct Pack<_Float16> {
+  static constexpr int N = 8;
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ uint4 empty() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+  static __device__ __forceinline__ void open(const uint4& w, float* f) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const h2 h = __builtin_bit_cast(h2, u[i]);
+      f[2 * i] = (float)h[0], f[2 * i + 1] = (float)h[1];
+    }
+  }
+  static __device__ __forceinline__ uint32_t two(float a, float b) { return __builtin_bit_cast(uint32_t, (h2){(_Float16)a, (_Float16)b}); }
+  static __device__ __forceinline__ uint4 close(const float* f) { return make_uint4(two(f[0], f[1]), two(f[2], f[3]), two(f[4], f[5]), two(f[6], f[7])); }
+};
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__hip_bfloat16 v) { return __bfloat162float(v); }
@@ -31,20 +88,23 @@ template <> __device__ __forceinline__ _Float16 from_float<_Float16>(float v) { 
 __device__ __forceinline__ float exp2_fast(float a) { return __builtin_amdgcn_exp2f(a); }
 __device__ __forceinline__ float log2_fast(float a) { return __builtin_amdgcn_logf(a); }
 __device__ __forceinline__ float nan_f() { return __builtin_nanf(""); }
-
 // (x - m) / T; halved first, for two finite scores may lie further apart than a float reaches while this does not
 __device__ __forceinline__ float below(float x, float m, float inv_t) { return (0.5f * x - 0.5f * m) * (2.f * inv_t); }
 
-// (max, sum of 2^a, sum of a 2^a); a is clamped where its power is 0 anyway, so that 0 * -inf never forms
+// ---- running sums ----------------------------------------------------------------------------------------------------------------
+// (max, sum of 2^a, sum of a 2^a); a is clamped where its power is 0 anyway, so that 0 * -inf never forms (a NaN reaches s unclamped)
 struct Sum {
   float m, s, t;
 };
-__device__ __forceinline__ float clamped(float a) { return a < -200.f ? -200.f : a; }  // (NaN stays)
+__device__ __forceinline__ float clamped(float a) { return fmaxf(a, -200.f); }
+__device__ __forceinline__ Sum moved(Sum v, float m, float c) {
+  const float d = clamped((v.m - m) * c), r = exp2_fast(d);
+  return Sum{m, v.s * r, r * (v.t + v.s * d)};
+}
 __device__ __forceinline__ Sum merge(Sum a, Sum b, float c) {
   const float m = fmaxf(a.m, b.m);
-  const float da = clamped((a.m - m) * c), db = clamped((b.m - m) * c);
-  const float ea = exp2_fast(da), eb = exp2_fast(db);
-  return Sum{m, a.s * ea + b.s * eb, ea * (a.t + a.s * da) + eb * (b.t + b.s * db)};
+  a = moved(a, m, c), b = moved(b, m, c);
+  return Sum{m, a.s + b.s, a.t + b.t};
 }
 __device__ __forceinline__ Sum wave_merge(Sum v, float c) {
 #pragma unroll
@@ -52,22 +112,95 @@ __device__ __forceinline__ Sum wave_merge(Sum v, float c) {
   return v;
 }
 
+// ---- best alternatives -------------------------------------------------------------------------------------------------------------
 // orders scores by value, then by lowest class; 0 is below every finite score
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t j) {
-  const uint32_t b = __float_as_uint(x + 0.f);  // (-0 becomes +0)
-  return ((uint64_t)(b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u)) << 32) | (uint32_t)~j;
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
-__device__ __forceinline__ float value_of(uint64_t key) {
-  const uint32_t o = (uint32_t)(key >> 32);
-  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t j) { return ((uint64_t)ordered(x + 0.f) << 32) | (uint32_t)~j; }  // (-0 becomes +0)
+__device__ __forceinline__ float value_of(uint64_t key) { return unordered((uint32_t)(key >> 32)); }
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) { return __shfl_xor((unsigned long long)v, d); }
+
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+  __builtin_amdgcn_wave_barrier();
 }
 
+// a lower bound, good to 16 bits, of the r-th largest of the lanes' values: bit by bit, by counting lanes
+__device__ __forceinline__ float rth_largest(float v, int r) {
+  const uint32_t o = ordered(v);
+  uint32_t t = 0;
+#pragma unroll
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t u = t | (1u << b);
+    if (__popcll(__ballot(o >= u)) >= r) t = u;
+  }
+  return t <= ordered(kLowest) ? kLowest : unordered(t);
+}
+
+// 64 keys across the lanes, falling
+__device__ __forceinline__ uint64_t sort64(uint64_t v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j >= 1; j >>= 1) {
+      const uint64_t o = shfl_xor64(v, j);
+      const bool keep_max = ((lane & j) == 0) == ((lane & k) == 0);
+      v = (o > v) == keep_max ? o : v;
+    }
+  return v;
+}
+// the 64 best of two falling lists
+__device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b, int lane) {
+  const uint64_t r = __shfl((unsigned long long)b, 63 - lane);
+  uint64_t v = a > r ? a : r;
+#pragma unroll
+  for (int j = 32; j >= 1; j >>= 1) {
+    const uint64_t o = shfl_xor64(v, j);
+    v = (o > v) == ((lane & j) == 0) ? o : v;
+  }
+  return v;
+}
+
+// a wave's list: lane i holds the i-th best key seen (0: none)
+struct Best {
+  uint64_t mine;
+  uint64_t* buf;  // kBuf candidates in LDS
+  float bound;    // scores below it are not among the k best of the row
+  int waiting, k;
+
+  __device__ __forceinline__ void offer(float f, uint32_t j) {
+    const bool in = f >= bound;  // (false for NaN and -inf: the bound is finite)
+    const uint64_t who = __ballot(in);
+    if (who == 0) return;
+    if (in) buf[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key_of(f, j);
+    waiting += __popcll(who);
+  }
+  __device__ void take(int n, int lane) {  // the last n <= 64 waiting
+    wave_fence();
+    waiting -= n;
+    const uint64_t v = sort64(lane < n ? buf[waiting + lane] : 0, lane);
+    wave_fence();
+    mine = merge64(mine, v, lane);
+    const uint32_t o = __builtin_amdgcn_readlane((uint32_t)(mine >> 32), k - 1);
+    if (o) bound = fmaxf(bound, unordered(o));
+  }
+  __device__ __forceinline__ void settle(int lane) {
+    while (waiting >= 64) take(64, lane);
+  }
+};
+
+// ---- arguments ---------------------------------------------------------------------------------------------------------------------
 struct FwdArgs {
   const void* x;
   int64_t rows, stride;
-  int32_t classes;
+  int32_t classes, segments, per_segment;
   float c, inv_t;
   float* stats;
+  float4* part;     // [rows][segments] (m, s, t) of a segment
+  uint64_t* keys;   // [rows][segments][top]
   // readout
   const int64_t* labels;
   int64_t ignore;
@@ -77,78 +210,11 @@ struct FwdArgs {
   // distillation
   const int64_t* index;
   const void* value;
-  int32_t value_type, list, tail;
+  int32_t value_type, list;
   float *loss, *q;
 };
 
-template <typename T>
-__device__ Sum row_sum(const T* x, int n, float c, Sum* red) {
-  Sum v{kLowest, 0.f, 0.f};
-  for (int j = threadIdx.x; j < n; j += kThreads) {
-    const float f = to_float(x[j]);
-    if (f > v.m) {
-      const float d = clamped((v.m - f) * c), r = exp2_fast(d);
-      v = Sum{f, v.s * r, r * (v.t + v.s * d)};
-    }
-    const float a = clamped((f - v.m) * c), e = exp2_fast(a);
-    v.s += e;
-    v.t += e * a;
-  }
-  v = wave_merge(v, c);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < kThreads / 64; ++w) v = merge(v, red[w], c);
-  return v;
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void readout_kernel(FwdArgs A) {
-  __shared__ Sum red[kThreads / 64];
-  __shared__ uint64_t best[kThreads / 64];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(A.x) + row * A.stride;
-  const int n = A.classes, tid = threadIdx.x;
-  const Sum v = row_sum(x, n, A.c, red);
-  const float l2 = log2_fast(v.s);
-  if (tid == 0) {
-    if (A.stats) reinterpret_cast<float4*>(A.stats)[row] = make_float4(v.m, v.s, v.t, 0.f);
-    if (A.lse) A.lse[row] = v.s == 0.f ? -INFINITY : v.m * A.inv_t + kLn2 * l2;
-    if (A.entropy) A.entropy[row] = v.s == 0.f ? 0.f : kLn2 * (l2 - v.t / v.s);
-    if (A.logprob) {
-      const int64_t y = A.labels[row];
-      float lp = nan_f();
-      if (y == A.ignore) lp = 0.f;
-      else if (y >= 0 && y < n) lp = v.s == 0.f ? -INFINITY : below(to_float(x[y]), v.m, A.inv_t) - kLn2 * l2;
-      A.logprob[row] = lp;
-    }
-  }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < A.top; ++k) {
-    uint64_t mine = 0;
-    for (int j = tid; j < n; j += kThreads) {
-      const float f = to_float(x[j]);
-      if (f >= kLowest) {
-        const uint64_t key = key_of(f, j);
-        if (key < last && key > mine) mine = key;
-      }
-    }
-    for (int d = 32; d >= 1; d >>= 1) {
-      const uint64_t o = __shfl_xor((unsigned long long)mine, d);
-      mine = o > mine ? o : mine;
-    }
-    __syncthreads();
-    if ((tid & 63) == 0) best[tid >> 6] = mine;
-    __syncthreads();
-    for (int w = 0; w < kThreads / 64; ++w) mine = best[w] > mine ? best[w] : mine;
-    last = mine;
-    if (tid == 0) {
-      const bool some = mine != 0 && v.s == v.s;
-      A.top_index[row * A.top + k] = some ? (int64_t)(uint32_t)~(uint32_t)mine : -1;
-      A.top_logprob[row * A.top + k] = v.s != v.s ? nan_f() : mine == 0 ? -INFINITY : below(value_of(mine), v.m, A.inv_t) - kLn2 * l2;
-    }
-  }
-}
+enum Mode { kReadout, kDistill, kDistillTail };
 
 __device__ __forceinline__ float load_value(const FwdArgs& A, int64_t i) {
   if (A.value_type == VITTA_SCORES_F32) return static_cast<const float*>(A.value)[i];
@@ -156,78 +222,323 @@ __device__ __forceinline__ float load_value(const FwdArgs& A, int64_t i) {
   return to_float(static_cast<const _Float16*>(A.value)[i]);
 }
 
+// ---- a row's answer, by one wave -----------------------------------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_kernel(FwdArgs A) {
-  __shared__ Sum red[kThreads / 64];
-  __shared__ int64_t idx[VITTA_SCORES_MAX_LIST];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(A.x) + row * A.stride;
-  const int n = A.classes, tid = threadIdx.x, K = A.list;
-  for (int k = tid; k < K; k += kThreads) {
-    const int64_t i = A.index[row * K + k];
-    idx[k] = i >= 0 && i < n ? i : -1;
-  }
-  __syncthreads();
-  Sum v = row_sum(x, n, A.c, red);
-  // what the classes outside the list hold: summed apart, for 1 minus the listed mass cancels
-  float rest = 0.f;
-  if (A.tail) {
-    for (int j = tid; j < n; j += kThreads) {
-      bool in = false;
-      for (int k = 0; k < K; ++k) in |= idx[k] == j;
-      if (!in) rest += exp2_fast((to_float(x[j]) - v.m) * A.c);
-    }
-    rest = wave_sum(rest);
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6].s = rest;
-    __syncthreads();
-    rest = 0.f;
-    for (int w = 0; w < kThreads / 64; ++w) rest += red[w].s;
-  }
-  if (tid != 0) return;
-  // the teacher's list and the loss, one thread
+__device__ void finish_readout(const FwdArgs& A, int64_t row, const T* x, Sum v, uint64_t mine, int lane) {
   const float l2 = log2_fast(v.s);
-  bool some = false;
-  float vm = kLowest, qs = 0.f;
-  for (int k = 0; k < K; ++k)
-    if (idx[k] >= 0) some = true, vm = fmaxf(vm, load_value(A, row * K + k));
-  const float cv = A.tail ? kLog2e : A.c;
-  const float ref = A.tail ? 0.f : vm;
-  for (int k = 0; k < K; ++k)
-    if (idx[k] >= 0) qs += exp2_fast((load_value(A, row * K + k) - ref) * cv);
-  const float ql2 = A.tail ? 0.f : log2_fast(qs), qinv = A.tail ? 1.f : 1.f / qs;
-  float loss = 0.f, sum = 0.f;
-  for (int k = 0; k < K; ++k) {
-    float q = 0.f;
-    if (idx[k] >= 0) {
-      const float b = (load_value(A, row * K + k) - ref) * cv;
-      q = exp2_fast(b) * qinv;
-      if (q != 0.f) {
-        const float log_q = A.tail ? load_value(A, row * K + k) : below(load_value(A, row * K + k), ref, A.inv_t) - kLn2 * ql2;
-        loss += q * (log_q - (v.s == 0.f ? -INFINITY : below(to_float(x[idx[k]]), v.m, A.inv_t) - kLn2 * l2));
-      }
-    }
-    sum += q;
-    A.q[row * K + k] = q;
-  }
-  float inside = some ? sum : 0.f, outside = inside;
-  if (A.tail && some) {
-    const float q_rest = fmaxf(1.f - sum, 0.f);
-    if (q_rest > 0.f && rest > 0.f) {
-      loss += q_rest * kLn2 * (log2_fast(q_rest) - log2_fast(rest / v.s));
-      inside = sum + q_rest;
-      outside = inside - q_rest * v.s / rest;
+  if (lane == 0) {
+    if (A.stats) reinterpret_cast<float4*>(A.stats)[row] = make_float4(v.m, v.s, v.t, 0.f);
+    if (A.lse) A.lse[row] = v.s == 0.f ? -INFINITY : v.m * A.inv_t + kLn2 * l2;
+    if (A.entropy) A.entropy[row] = v.s == 0.f ? 0.f : kLn2 * (l2 - v.t / v.s);
+    if (A.logprob) {
+      const int64_t y = A.labels[row];
+      float lp = nan_f();
+      if (y == A.ignore) lp = 0.f;
+      else if (y >= 0 && y < A.classes) lp = v.s == 0.f ? -INFINITY : below(to_float(x[y]), v.m, A.inv_t) - kLn2 * l2;
+      A.logprob[row] = lp;
     }
   }
-  A.loss[row] = some ? loss : 0.f;
-  reinterpret_cast<float4*>(A.stats)[row] = make_float4(v.m, v.s, inside, outside);
+  if (lane < A.top) {
+    const bool whole = v.s == v.s;
+    A.top_index[row * A.top + lane] = mine != 0 && whole ? (int64_t)(uint32_t)~(uint32_t)mine : -1;
+    A.top_logprob[row * A.top + lane] = !whole ? nan_f() : mine == 0 ? -INFINITY : below(value_of(mine), v.m, A.inv_t) - kLn2 * l2;
+  }
 }
 
+// v: the row's sums, without the listed classes where these are one side of a tail
+template <typename T, bool TAIL>
+__device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v, int lane) {
+  constexpr int R = VITTA_SCORES_MAX_LIST / 64;
+  const int K = A.list;
+  int32_t at[R];
+  float val[R], z[R];
+  bool some = false;
+  float vm = kLowest;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int k = i * 64 + lane;
+    at[i] = -1;
+    if (k < K) {
+      const int64_t j = A.index[row * K + k];
+      if (j >= 0 && j < A.classes) at[i] = (int32_t)j;
+    }
+    val[i] = at[i] >= 0 ? load_value(A, row * K + k) : -INFINITY;
+    z[i] = at[i] >= 0 ? to_float(x[at[i]]) : -INFINITY;
+    some |= at[i] >= 0;
+    vm = fmaxf(vm, val[i]);
+  }
+  some = __ballot(some) != 0;
+  float m = v.m, s = v.s, rest = 0.f;
+  if (TAIL) {  // the listed classes' own sum, each once
+    uint32_t again = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int n = min(64, K - i * 64);
+      for (int l = 0; l < n; ++l) {
+        const int32_t j = __builtin_amdgcn_readlane(at[i], l);
+#pragma unroll
+        for (int o = 0; o < R; ++o)
+          if (at[o] == j && o * 64 + lane > i * 64 + l) again |= 1u << o;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) m = fmaxf(m, z[i]);
+    m = wave_max(m);
+    float in = 0.f;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (at[i] >= 0 && !(again >> i & 1)) in += exp2_fast((z[i] - m) * A.c);
+    rest = v.s * exp2_fast((v.m - m) * A.c);
+    s = rest + wave_sum(in);
+  }
+  const float l2 = log2_fast(s);
+  const float ref = TAIL ? 0.f : wave_max(vm), cv = TAIL ? kLog2e : A.c;
+  float q[R], sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    q[i] = at[i] >= 0 ? exp2_fast((val[i] - ref) * cv) : 0.f;
+    sum += q[i];
+  }
+  sum = wave_sum(sum);
+  const float inv = TAIL ? 1.f : 1.f / sum, ql = TAIL ? 0.f : kLn2 * log2_fast(sum);
+  float loss = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int k = i * 64 + lane;
+    if (at[i] >= 0) {
+      q[i] *= inv;
+      if (q[i] != 0.f) {
+        const float log_q = TAIL ? val[i] : below(val[i], ref, A.inv_t) - ql;
+        loss += q[i] * (log_q - (s == 0.f ? -INFINITY : below(z[i], m, A.inv_t) - kLn2 * l2));
+      }
+    }
+    if (k < K) A.q[row * K + k] = q[i];
+  }
+  loss = wave_sum(loss);
+  if (lane != 0) return;
+  float inside = !some ? 0.f : TAIL ? sum : 1.f, outside = inside;
+  if (TAIL && some) {
+    const float q_rest = fmaxf(1.f - sum, 0.f);
+    if (q_rest > 0.f && rest > 0.f) {
+      loss += q_rest * kLn2 * (log2_fast(q_rest) - log2_fast(rest / s));
+      inside = sum + q_rest;
+      outside = inside - q_rest * s / rest;
+    }
+    if (sum != sum || s != s) loss = nan_f();  // (comparisons with a NaN are false)
+  }
+  A.loss[row] = some ? loss : 0.f;
+  reinterpret_cast<float4*>(A.stats)[row] = make_float4(m, s, inside, outside);
+}
+
+// ---- forward ---------------------------------------------------------------------------------------------------------------------------
+// NW waves share a (segment of a) row; with NW == 1 the four waves of a workgroup take four rows.
+template <typename T, int NW, int MODE, bool ENT, bool TOP>
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdArgs A) {
+  constexpr int N = Pack<T>::N, NT = NW * 64, G = NW == 1 ? 4 : 1;  // G groups in a workgroup
+  extern __shared__ __attribute__((aligned(16))) uint32_t bits_all[];  // kDistillTail: one bit per class of the group's segment
+  __shared__ uint64_t buf[TOP ? (NW == 1 ? 4 : NW) * kBuf : 1];
+  __shared__ Sum red[NW];
+  __shared__ float bounds[NW];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = NW == 1 ? lane : threadIdx.x;
+  int64_t row;
+  int seg = 0;
+  if (NW == 1) {
+    row = (int64_t)blockIdx.x * G + wave;
+    if (row >= A.rows) return;  // (no workgroup barrier in this form)
+  } else if (A.segments == 1) {
+    row = blockIdx.x;
+  } else {
+    row = blockIdx.x / A.segments;
+    seg = blockIdx.x - (int)row * A.segments;
+  }
+  const T* whole = static_cast<const T*>(A.x) + row * A.stride;
+  const int j0 = seg * A.per_segment, n = min(A.per_segment, A.classes - j0);
+  const T* x = whole + j0;
+  const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+  const int nv = (n - head) / N, body = head + nv * N;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+
+  uint32_t* bits = bits_all;
+  if (MODE == kDistillTail) {  // class j0 + i at bit i - head + 16: a vector's bits never straddle a byte
+    const int words = (A.per_segment + 16 + 31) / 32 + 1;
+    bits += (NW == 1 ? wave : 0) * words;
+    for (int i = tid; i < words; i += NT) bits[i] = 0;
+    if (NW > 1) __syncthreads(); else wave_fence();
+    for (int k = tid; k < A.list; k += NT) {
+      const int64_t j = A.index[row * A.list + k] - j0;
+      if (j >= 0 && j < n) atomicOr(&bits[(j - head + 16) >> 5], 1u << ((j - head + 16) & 31));
+    }
+    if (NW > 1) __syncthreads(); else wave_fence();
+  }
+
+  Sum v{kLowest, 0.f, 0.f};
+  Best best{0, buf + (TOP ? wave * kBuf : 0), kLowest, 0, A.top};
+  const float c = A.c;
+
+  // the vectors at + u * NT of this lane (those from nv on are empty)
+  auto load = [&](uint4* w, int at) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) w[u] = at + u * NT < nv ? xv[at + u * NT] : Pack<T>::empty();
+  };
+  auto consume = [&](const uint4* w, int base, bool first) {
+    float f[kU][N], cu[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      cu[u] = -INFINITY;
+      if (base + u * NT >= nv) continue;  // (the same for the whole group)
+      Pack<T>::open(w[u], f[u]);
+      if (MODE == kDistillTail) {
+        const int at = base + u * NT + tid;
+        uint32_t in = 0;
+        if (at < nv) in = reinterpret_cast<const uint8_t*>(bits)[2 + (N == 8 ? at : at >> 1)];
+        if (N == 4) in = (at & 1) ? in >> 4 : in & 15;
+        if (in) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) f[u][i] = in >> i & 1 ? -INFINITY : f[u][i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) cu[u] = fmaxf(cu[u], f[u][i]);
+    }
+    float cm = cu[0];
+#pragma unroll
+    for (int u = 1; u < kU; ++u) cm = fmaxf(cm, cu[u]);
+    const float m = fmaxf(v.m, cm);
+    if (ENT) {
+      v = moved(v, m, c);
+    } else {
+      v.s *= exp2_fast((v.m - m) * c);
+      v.m = m;
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (base + u * NT >= nv) continue;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float a = (f[u][i] - m) * c, e = exp2_fast(a);
+        v.s += e;
+        if (ENT) v.t = fmaf(e, clamped(a), v.t);
+      }
+    }
+    if (TOP) {
+      if (first) {  // every wave has r maxima at or above its bound: NW r >= k scores of the row are
+        best.bound = rth_largest(cm, (A.top + NW - 1) / NW);
+        if (NW > 1) {
+          if (lane == 0) bounds[wave] = best.bound;
+          __syncthreads();
+#pragma unroll
+          for (int o = 0; o < NW; ++o) best.bound = fminf(best.bound, bounds[o]);
+        }
+      }
+      if (__ballot(cm >= best.bound) != 0) {
+        uint32_t which = 0;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) which |= __ballot(cu[u] >= best.bound) != 0 ? 1u << u : 0u;
+        while (which) {
+          const int u = __builtin_ctz(which), at = base + u * NT + tid;
+          which &= which - 1;
+          float g[N];
+          Pack<T>::open(at < nv ? xv[at] : Pack<T>::empty(), g);  // (again: an index into registers has to be a constant)
+#pragma unroll
+          for (int i = 0; i < N; ++i) best.offer(g[i], (uint32_t)(j0 + head + at * N + i));
+          best.settle(lane);
+        }
+      }
+    }
+  };
+
+  uint4 now[kU], next[kU];
+  load(now, tid);
+  const int steps = max(1, (nv + kU * NT - 1) / (kU * NT));
+  for (int step = 0; step < steps; ++step) {
+    const int base = step * kU * NT;
+    if (step + 1 < steps) load(next, base + kU * NT + tid);
+    consume(now, base, step == 0);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) now[u] = next[u];
+  }
+  // what lies before the first and behind the last whole vector: at most 2 (N - 1) <= 14 elements, one a lane
+  if (NW == 1 || wave == 0) {
+    const int rest = n - nv * N, i = lane < head ? lane : body + lane - head;
+    if (rest > 0) {
+      float f = lane < rest ? to_float(x[i]) : -INFINITY;
+      if (TOP) best.offer(f, (uint32_t)(j0 + i));
+      if (MODE == kDistillTail && lane < rest && (bits[(i - head + 16) >> 5] >> ((i - head + 16) & 31) & 1)) f = -INFINITY;
+      v = moved(v, fmaxf(v.m, f), c);
+      const float a = (f - v.m) * c, e = exp2_fast(a);
+      v.s += e;
+      v.t = fmaf(e, clamped(a), v.t);
+    }
+  }
+  v = wave_merge(v, c);
+  if (TOP) {
+    best.settle(lane);
+    if (best.waiting) best.take(best.waiting, lane);
+  }
+  if (NW > 1) {
+    if (lane == 0) red[wave] = v;
+    if (TOP) best.buf[lane] = best.mine;
+    __syncthreads();
+    if (TOP) {
+      for (int d = 1; d < NW; d <<= 1) {
+        if ((wave & (2 * d - 1)) == 0) {
+          best.mine = merge64(best.mine, best.buf[d * kBuf + lane], lane);
+          best.buf[lane] = best.mine;
+        }
+        __syncthreads();
+      }
+    }
+    if (wave != 0) return;
+    v = lane < NW ? red[lane] : Sum{kLowest, 0.f, 0.f};
+#pragma unroll
+    for (int d = NW / 2; d >= 1; d >>= 1) v = merge(v, Sum{__shfl_xor(v.m, d), __shfl_xor(v.s, d), __shfl_xor(v.t, d)}, c);
+    v.m = __shfl(v.m, 0), v.s = __shfl(v.s, 0), v.t = __shfl(v.t, 0);
+    if (A.segments > 1) {
+      const int64_t at = row * A.segments + seg;
+      if (lane == 0) A.part[at] = make_float4(v.m, v.s, v.t, 0.f);
+      if (TOP && lane < A.top) A.keys[at * A.top + lane] = best.mine;
+      return;
+    }
+  }
+  if (MODE == kReadout) finish_readout<T>(A, row, whole, v, best.mine, lane);
+  else finish_distill<T, MODE == kDistillTail>(A, row, whole, v, lane);
+}
+
+// joins the segments of a row: four waves merge the lists, the first one the sums
+template <typename T, int MODE, bool TOP>
+__global__ __launch_bounds__(256) void scores_join_kernel(FwdArgs A) {
+  __shared__ uint64_t lists[4 * 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(A.x) + row * A.stride;
+  uint64_t mine = 0;
+  if (TOP) {
+    for (int s = wave; s < A.segments; s += 4) {
+      const uint64_t o = lane < A.top ? A.keys[(row * A.segments + s) * A.top + lane] : 0;
+      mine = merge64(mine, o, lane);
+    }
+    lists[threadIdx.x] = mine;
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  if (TOP)
+    for (int w = 1; w < 4; ++w) mine = merge64(mine, lists[w * 64 + lane], lane);
+  Sum v{kLowest, 0.f, 0.f};
+  if (lane < A.segments) {
+    const float4 p = A.part[row * A.segments + lane];
+    v = Sum{p.x, p.y, p.z};
+  }
+  v = wave_merge(v, A.c);
+  if (MODE == kReadout) finish_readout<T>(A, row, x, v, mine, lane);
+  else finish_distill<T, MODE == kDistillTail>(A, row, x, v, lane);
+}
+
+// ---- gradient --------------------------------------------------------------------------------------------------------------------------
 struct BwdArgs {
   const void* x;
   void* dx;
   int64_t rows, stride;
-  int32_t classes;
+  int32_t classes, segments, per_segment;
   float c, inv_t;
   const float* stats;
   const int64_t* labels;
@@ -242,61 +553,123 @@ struct BwdArgs {
   int64_t s_g;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void readout_grad_kernel(BwdArgs A) {
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(A.x) + row * A.stride;
-  T* dx = static_cast<T*>(A.dx) + row * (int64_t)A.classes;
+// dx_j = e_j (a0 + a1 a_j), with a0 = at0 for the classes of the group's list, to which it adds `add`
+template <typename T, int NT, bool DISTILL, bool ENT>
+__global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
+  constexpr int N = Pack<T>::N, G = 256 / NT, L = DISTILL ? VITTA_SCORES_MAX_LIST : VITTA_SCORES_MAX_TOP + 1;
+  __shared__ int32_t at_all[G * L];
+  __shared__ float add_all[G * L];
+  const int group = threadIdx.x / NT, tid = threadIdx.x - group * NT, lane = threadIdx.x & 63;
+  int32_t* at = at_all + group * L;
+  float* add = add_all + group * L;
+  const int64_t unit = (int64_t)blockIdx.x * G + group;
+  const int64_t row = A.segments == 1 ? unit : unit / A.segments;
+  if (row >= A.rows) return;  // (G > 1 only: a wave for itself)
+  const int seg = A.segments == 1 ? 0 : (int)(unit - row * A.segments);
+  const int j0 = seg * A.per_segment, n = min(A.per_segment, A.classes - j0);
+  const T* x = static_cast<const T*>(A.x) + row * A.stride + j0;
+  T* dx = static_cast<T*>(A.dx) + row * (int64_t)A.classes + j0;
+  const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
+  const int nv = (n - head) / N, body = head + nv * N;
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+
+  uint4 now[kU], next[kU];
+  auto load = [&](uint4* w, int i) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) w[u] = i + u * NT < nv ? xv[i + u * NT] : Pack<T>::empty();
+  };
+  load(now, tid);
+
   const float4 st = reinterpret_cast<const float4*>(A.stats)[row];
-  const float m = st.x, is = st.y == 0.f ? 0.f : 1.f / st.y;
-  const int64_t y = A.g_logprob ? A.labels[row] : -1;
-  const bool given = A.g_logprob && y != A.ignore;
-  float gl = given ? A.g_logprob[row * A.s_logprob] : 0.f;
-  if (given && (y < 0 || y >= A.classes)) gl = nan_f();
-  const float gh = A.g_entropy ? A.g_entropy[row * A.s_entropy] : 0.f;
-  float all = -gl + (A.g_lse ? A.g_lse[row * A.s_lse] : 0.f);
-  if (A.g_top)
-    for (int k = 0; k < A.top; ++k)
-      if (A.top_index[row * A.top + k] >= 0) all -= A.g_top[row * A.top + k];
-  // dx_j = (e_j / s) / T (all - g_H ln2 (a_j - t / s)) + what the label and the alternatives add
-  for (int j = threadIdx.x; j < A.classes; j += kThreads) {
-    const float a = clamped((to_float(x[j]) - m) * A.c);
-    float g = 0.f;
-    if (all != 0.f || gh != 0.f) g = exp2_fast(a) * is * (all - gh * kLn2 * (a - st.z * is));
-    if (given && j == y && st.y != 0.f) g += gl;
-    if (A.g_top)
-      for (int k = 0; k < A.top; ++k)
-        if (A.top_index[row * A.top + k] == j) g += A.g_top[row * A.top + k];
-    dx[j] = from_float<T>(g * A.inv_t);
+  const float m = st.x, is = st.y == 0.f ? 0.f : 1.f / st.y, c = A.c;
+  float a0, a1 = 0.f, at0;
+  int many;
+  if (DISTILL) {
+    const float g = A.g[row * A.s_g] * A.inv_t;
+    many = A.list;
+    for (int k = tid; k < many; k += NT) {
+      const int64_t j = A.index[row * A.list + k] - j0;
+      at[k] = j >= 0 && j < n ? (int32_t)j : -1;
+      add[k] = -g * A.q[row * A.list + k];
+    }
+    at0 = st.z == 0.f || g == 0.f ? 0.f : g * is * st.z;
+    a0 = st.w == 0.f || g == 0.f ? 0.f : g * is * st.w;
+  } else {
+    const int64_t y = A.g_logprob ? A.labels[row] : A.ignore;
+    float gl = y != A.ignore ? A.g_logprob[row * A.s_logprob] : 0.f;
+    if (y != A.ignore && (y < 0 || y >= A.classes)) gl = nan_f();
+    const float gh = ENT ? A.g_entropy[row * A.s_entropy] : 0.f;
+    float all = (A.g_lse ? A.g_lse[row * A.s_lse] : 0.f) - gl;
+    many = 1;
+    if (A.g_top) {
+      many += A.top;
+      float sum = 0.f;
+      for (int k = lane; k < A.top; k += 64) {  // (every wave the whole list: all of them need the sum)
+        const int64_t j = A.top_index[row * A.top + k];
+        const float g = A.g_top[row * A.top + k];
+        if (j >= 0) sum += g;
+        if (tid < 64) {
+          at[1 + k] = j >= j0 && j < j0 + (int64_t)n ? (int32_t)(j - j0) : -1;
+          add[1 + k] = g * A.inv_t;
+        }
+      }
+      all -= wave_sum(sum);
+    }
+    if (tid == 0) {
+      at[0] = y != A.ignore && y >= j0 && y < j0 + (int64_t)n ? (int32_t)(y - j0) : -1;
+      add[0] = st.y == 0.f ? 0.f : gl * A.inv_t;
+    }
+    a0 = is * A.inv_t * (all + (ENT ? gh * kLn2 * st.z * is : 0.f));
+    a1 = ENT ? -is * A.inv_t * gh * kLn2 : 0.f;
+    if (all == 0.f && gh == 0.f) a0 = a1 = 0.f;
+    at0 = a0;
+  }
+  const bool dead = a0 == 0.f && a1 == 0.f;  // zeros whatever the row holds
+  auto grad = [&](float f, float b) {
+    const float a = (f - m) * c, e = exp2_fast(a);
+    return e * (ENT ? fmaf(a1, clamped(a), b) : b);
+  };
+
+  const bool straight = (reinterpret_cast<uintptr_t>(dx + head) & 15) == 0;
+  const int steps = (nv + kU * NT - 1) / (kU * NT);
+  for (int step = 0; step < steps; ++step) {
+    const int base = step * kU * NT + tid;
+    if (step + 1 < steps) load(next, base + kU * NT);
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int i = base + u * NT;
+      if (i < nv) {
+        float f[N];
+        Pack<T>::open(now[u], f);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = dead ? 0.f : grad(f[e], a0);
+        const uint4 w = Pack<T>::close(f);
+        if (straight) {
+          reinterpret_cast<uint4*>(dx + head)[i] = w;
+        } else {
+          __builtin_memcpy(__builtin_assume_aligned(dx + head + (int64_t)i * N, sizeof(T)), &w, 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) now[u] = next[u];
+  }
+  if (tid < n - nv * N) {
+    const int i = tid < head ? tid : body + tid - head;
+    dx[i] = from_float<T>(dead ? 0.f : grad(to_float(x[i]), a0));
+  }
+  // the listed classes again, each with all that is added to it
+  if (NT > 64) __syncthreads(); else wave_fence();
+  for (int k = tid; k < many; k += NT) {
+    const int j = at[k];
+    if (j < 0) continue;
+    float sum = 0.f;
+    for (int o = 0; o < many; ++o) sum += at[o] == j ? add[o] : 0.f;
+    dx[j] = from_float<T>((at0 == 0.f && a1 == 0.f ? 0.f : grad(to_float(x[j]), at0)) + sum);
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_grad_kernel(BwdArgs A) {
-  __shared__ int64_t idx[VITTA_SCORES_MAX_LIST];
-  __shared__ float q[VITTA_SCORES_MAX_LIST];
-  const int64_t row = blockIdx.x;
-  const int K = A.list;
-  for (int k = threadIdx.x; k < K; k += kThreads) {
-    idx[k] = A.index[row * K + k];
-    q[k] = A.q[row * K + k];
-  }
-  __syncthreads();
-  const T* x = static_cast<const T*>(A.x) + row * A.stride;
-  T* dx = static_cast<T*>(A.dx) + row * (int64_t)A.classes;
-  const float4 st = reinterpret_cast<const float4*>(A.stats)[row];
-  const float is = st.y == 0.f ? 0.f : 1.f / st.y, g = A.g[row * A.s_g] * A.inv_t;
-  for (int j = threadIdx.x; j < A.classes; j += kThreads) {
-    float pull = 0.f;
-    bool in = false;
-    for (int k = 0; k < K; ++k)
-      if (idx[k] == j) pull += q[k], in = true;
-    const float f = in ? st.z : st.w;
-    const float p = f == 0.f ? 0.f : exp2_fast((to_float(x[j]) - st.x) * A.c) * is * f;
-    dx[j] = from_float<T>(g * (p - pull));
-  }
-}
-
+// ---- launches ----------------------------------------------------------------------------------------------------------------------------
 bool bad_stats(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15u); }
 bool bad_out(const void* p, int32_t type) { return !p || reinterpret_cast<uintptr_t>(p) % (type == VITTA_SCORES_F32 ? 4 : 2); }
 
@@ -306,19 +679,86 @@ bool bad_scores(const void* x, int32_t type, int64_t rows, int32_t classes, int6
   return reinterpret_cast<uintptr_t>(x) % (type == VITTA_SCORES_F32 ? 4 : 2) != 0;
 }
 
-#define SCORES_LAUNCH(kernel, type, args)                                                                                    \
-  do {                                                                                                                       \
-    const dim3 grid((unsigned)(args).rows);                                                                                  \
-    if ((type) == VITTA_SCORES_F32) VITTA_LAUNCH(kernel<float>, grid, dim3(kThreads), 0, st, args);                          \
-    else if ((type) == VITTA_SCORES_BF16) VITTA_LAUNCH(kernel<__hip_bfloat16>, grid, dim3(kThreads), 0, st, args);           \
-    else VITTA_LAUNCH(kernel<_Float16>, grid, dim3(kThreads), 0, st, args);                                                  \
-  } while (0)
+struct Cut {
+  int32_t segments, per_segment;
+};
+Cut cut_into(int32_t classes, int64_t segments) {
+  int64_t per = (classes + segments - 1) / segments;
+  per = (per + 511) / 512 * 512;  // (whole 16-byte vectors: a segment starts as the row is aligned)
+  return Cut{(int32_t)((classes + per - 1) / per), (int32_t)per};
+}
+// Segments of a row in the forward: enough workgroups for the chip, none of fewer than 8192 classes.
+Cut fwd_cut(int64_t rows, int32_t classes) {
+  if (classes <= kWaveRow) return Cut{1, classes};
+  int64_t s = (512 + rows - 1) / rows;
+  s = s < classes / 8192 ? s : classes / 8192;
+  s = s > kMaxSegments ? kMaxSegments : s;
+  const int64_t least = ((int64_t)classes + kTailSegment - 1) / kTailSegment;  // (membership bits)
+  s = s < least ? least : s;
+  return s <= 1 ? Cut{1, classes} : cut_into(classes, s);
+}
+// A workgroup of the gradient takes 16384 classes of a row.
+Cut bwd_cut(int32_t classes) { return classes <= 16384 ? Cut{1, classes} : cut_into(classes, ((int64_t)classes + 16383) / 16384); }
+
+// sizes a launch does not take: more workgroups than a grid has, rows that no 64 segments of kTailSegment hold
+bool too_large(int64_t rows, int32_t classes) {
+  if (classes > kMaxSegments * kTailSegment || rows > 0x7fffffff) return true;
+  return rows * (int64_t)fwd_cut(rows, classes).segments > 0x7fffffff || rows * (int64_t)bwd_cut(classes).segments > 0x7fffffff;
+}
+
+template <typename T, int MODE, bool ENT, bool TOP>
+int launch_fwd(FwdArgs a, void* ws, hipStream_t st) {
+  const Cut cut = fwd_cut(a.rows, a.classes);
+  a.segments = cut.segments, a.per_segment = cut.per_segment;
+  const size_t bits = MODE == kDistillTail ? ((size_t)(cut.per_segment + 16 + 31) / 32 + 1) * 4 : 0;
+  if (a.classes <= kWaveRow) {
+    VITTA_LAUNCH((scores_kernel<T, 1, MODE, ENT, TOP>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 4 * bits, st, a);
+    return VITTA_OK;
+  }
+  if (cut.segments > 1) {
+    a.part = static_cast<float4*>(ws);
+    a.keys = reinterpret_cast<uint64_t*>(a.part + a.rows * cut.segments);
+  }
+  VITTA_LAUNCH((scores_kernel<T, kWaves, MODE, ENT, TOP>), dim3((unsigned)(a.rows * cut.segments)), dim3(kWaves * 64), bits, st, a);
+  if (cut.segments > 1) VITTA_LAUNCH((scores_join_kernel<T, MODE, TOP>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  return VITTA_OK;
+}
+
+template <int MODE, bool ENT, bool TOP>
+int launch_fwd(int32_t type, const FwdArgs& a, void* ws, void* stream) {
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (type == VITTA_SCORES_F32) return launch_fwd<float, MODE, ENT, TOP>(a, ws, st);
+  if (type == VITTA_SCORES_BF16) return launch_fwd<__hip_bfloat16, MODE, ENT, TOP>(a, ws, st);
+  return launch_fwd<_Float16, MODE, ENT, TOP>(a, ws, st);
+}
+
+template <typename T, bool DISTILL, bool ENT>
+int launch_bwd(BwdArgs a, hipStream_t st) {
+  const Cut cut = bwd_cut(a.classes);
+  a.segments = cut.segments, a.per_segment = cut.per_segment;
+  const int64_t units = a.rows * cut.segments;
+  if (a.classes <= kWaveRow) VITTA_LAUNCH((scores_grad_kernel<T, 64, DISTILL, ENT>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
+  else VITTA_LAUNCH((scores_grad_kernel<T, 256, DISTILL, ENT>), dim3((unsigned)units), dim3(256), 0, st, a);
+  return VITTA_OK;
+}
+
+template <bool DISTILL, bool ENT>
+int launch_bwd(int32_t type, const BwdArgs& a, void* stream) {
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (type == VITTA_SCORES_F32) return launch_bwd<float, DISTILL, ENT>(a, st);
+  if (type == VITTA_SCORES_BF16) return launch_bwd<__hip_bfloat16, DISTILL, ENT>(a, st);
+  return launch_bwd<_Float16, DISTILL, ENT>(a, st);
+}
 
 }  // namespace
 
 extern "C" {
 
-size_t vitta_scores_workspace_bytes(int64_t, int32_t, int32_t, int32_t) { return 0; }
+size_t vitta_scores_workspace_bytes(int64_t rows, int32_t classes, int32_t, int32_t top) {
+  if (rows <= 0 || classes <= 0 || top < 0 || top > VITTA_SCORES_MAX_TOP || too_large(rows, classes)) return 0;
+  const int64_t s = fwd_cut(rows, classes).segments;
+  return s == 1 ? 0 : (size_t)rows * s * (16 + 8 * (size_t)top);
+}
 
 int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
                              const int64_t* d_labels, int64_t ignore_index, int32_t top, float* d_logprob, float* d_entropy,
@@ -328,16 +768,15 @@ int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32
   if (top < 0 || top > VITTA_SCORES_MAX_TOP || top > classes || (top > 0 && (!d_top_logprob || !d_top_index))) return VITTA_ERR_INVALID_ARG;
   if (!d_labels != !d_logprob || (!d_logprob && !d_entropy && !d_lse && top == 0)) return VITTA_ERR_INVALID_ARG;
   if (d_stats && bad_stats(d_stats)) return VITTA_ERR_INVALID_ARG;
-  if (rows > 0x7fffffff) return VITTA_ERR_UNSUPPORTED;
-  if (workspace_bytes < vitta_scores_workspace_bytes(rows, classes, dtype, top)) return VITTA_ERR_WORKSPACE;
-  (void)d_workspace;
+  if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
+  const size_t need = vitta_scores_workspace_bytes(rows, classes, dtype, top);
+  if (workspace_bytes < need || (need && bad_stats(d_workspace))) return VITTA_ERR_WORKSPACE;
   FwdArgs a{};
   a.x = d_x, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.labels = d_labels, a.ignore = ignore_index, a.top = top, a.logprob = d_logprob, a.entropy = d_entropy, a.lse = d_lse;
   a.top_logprob = d_top_logprob, a.top_index = d_top_index;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  SCORES_LAUNCH(readout_kernel, dtype, a);
-  return VITTA_OK;
+  if (d_entropy) return top ? launch_fwd<kReadout, true, true>(dtype, a, d_workspace, stream) : launch_fwd<kReadout, true, false>(dtype, a, d_workspace, stream);
+  return top ? launch_fwd<kReadout, false, true>(dtype, a, d_workspace, stream) : launch_fwd<kReadout, false, false>(dtype, a, d_workspace, stream);
 }
 
 int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
@@ -347,15 +786,13 @@ int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32
                              void* stream) {
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature) || bad_stats(d_stats) || bad_out(d_dx, dtype)) return VITTA_ERR_INVALID_ARG;
   if ((d_glogprob && !d_labels) || (d_gtop && (!d_top_index || top <= 0 || top > VITTA_SCORES_MAX_TOP))) return VITTA_ERR_INVALID_ARG;
-  if (rows > 0x7fffffff) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   BwdArgs a{};
   a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.labels = d_labels, a.ignore = ignore_index, a.top = top, a.top_index = d_top_index;
   a.g_logprob = d_glogprob, a.g_entropy = d_gentropy, a.g_lse = d_glse, a.g_top = d_gtop;
   a.s_logprob = glogprob_stride, a.s_entropy = gentropy_stride, a.s_lse = glse_stride;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  SCORES_LAUNCH(readout_grad_kernel, dtype, a);
-  return VITTA_OK;
+  return d_gentropy ? launch_bwd<false, true>(dtype, a, stream) : launch_bwd<false, false>(dtype, a, stream);
 }
 
 int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
@@ -364,16 +801,14 @@ int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t 
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || !d_value || !d_loss || bad_stats(d_stats) || !d_q || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
   if (value_dtype < VITTA_SCORES_F32 || value_dtype > VITTA_SCORES_F16) return VITTA_ERR_INVALID_ARG;
-  if (rows > 0x7fffffff) return VITTA_ERR_UNSUPPORTED;
-  if (workspace_bytes < vitta_scores_workspace_bytes(rows, classes, dtype, 0)) return VITTA_ERR_WORKSPACE;
-  (void)d_workspace;
+  if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
+  const size_t need = vitta_scores_workspace_bytes(rows, classes, dtype, 0);
+  if (workspace_bytes < need || (need && bad_stats(d_workspace))) return VITTA_ERR_WORKSPACE;
   FwdArgs a{};
   a.x = d_x, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
-  a.stats = d_stats, a.index = d_index, a.value = d_value, a.value_type = value_dtype, a.list = list, a.tail = tail != 0;
+  a.stats = d_stats, a.index = d_index, a.value = d_value, a.value_type = value_dtype, a.list = list;
   a.loss = d_loss, a.q = d_q;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  SCORES_LAUNCH(distill_kernel, dtype, a);
-  return VITTA_OK;
+  return tail ? launch_fwd<kDistillTail, false, false>(dtype, a, d_workspace, stream) : launch_fwd<kDistill, false, false>(dtype, a, d_workspace, stream);
 }
 
 int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
@@ -381,13 +816,11 @@ int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t 
                           int64_t g_stride, void* d_dx, void* stream) {
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || bad_stats(d_stats) || !d_q || !d_g || bad_out(d_dx, dtype) || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
-  if (rows > 0x7fffffff) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   BwdArgs a{};
   a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.index = d_index, a.list = list, a.q = d_q, a.g = d_g, a.s_g = g_stride;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  SCORES_LAUNCH(distill_grad_kernel, dtype, a);
-  return VITTA_OK;
+  return launch_bwd<true, false>(dtype, a, stream);
 }
 
 }  // extern "C"
