@@ -49,7 +49,8 @@ def _check_readout(got, x, labels, top, temperature, ignore_index=-100):
         _close(got.logprob, o["logprob"], b_lp(o["logprob"]), "logprob")
     if got.entropy is not None:
         _close(got.entropy, o["entropy"], b_h, "entropy")
-    _close(got.lse, o["lse"], b_lse, "lse")
+    if got.lse is not None:
+        _close(got.lse, o["lse"], b_lse, "lse")
     if top:
         assert torch.equal(got.top_index.cpu(), o["top_index"]), "top_index"
         _close(got.top_logprob, o["top_logprob"], b_lp(o["top_logprob"]), "top_logprob")
@@ -68,18 +69,19 @@ def test_readout(rows, classes, top, dtype):
         dx, x = _scores(rows, classes, dtype, classes + rows, pad, start)
         labels = torch.randint(classes, (rows,), generator=torch.Generator().manual_seed(rows))
         labels[rows // 2] = -100
-        got = ops.label_logprobs(dx, labels.to(DEV), top=top, temperature=temperature)
+        got = ops.label_logprobs(dx, labels.to(DEV), top=top, lse=True, temperature=temperature)
         _check_readout(got, x, labels, top, temperature)
 
 
 def test_readout_parts_that_are_not_asked():
     from vitta_amd import ops
     dx, x = _scores(4, 300, torch.float32, 1)
-    a = ops.label_logprobs(dx)
+    a = ops.label_logprobs(dx, lse=True)
     assert a.logprob is None and a.top_index is None and a.top_logprob is None
     b = ops.label_logprobs(dx, torch.zeros(4, dtype=torch.int32, device=DEV), entropy=False, top=2)
     assert b.entropy is None
-    full = ops.label_logprobs(dx, torch.zeros(4, dtype=torch.int64, device=DEV), top=2)
+    assert b.lse is None
+    full = ops.label_logprobs(dx, torch.zeros(4, dtype=torch.int64, device=DEV), top=2, lse=True)
     assert torch.equal(a.entropy, full.entropy) and torch.equal(a.lse, full.lse)
     assert torch.equal(b.logprob, full.logprob) and torch.equal(b.top_index, full.top_index)
 
@@ -88,16 +90,16 @@ def test_readout_leading_dimensions_and_empty_ones():
     from vitta_amd import ops
     dx, x = _scores(12, 37, torch.bfloat16, 2)
     labels = torch.arange(12, device=DEV)
-    flat = ops.label_logprobs(dx, labels, top=3)
-    deep = ops.label_logprobs(dx.view(2, 3, 2, 37), labels.view(2, 3, 2), top=3)
+    flat = ops.label_logprobs(dx, labels, top=3, lse=True)
+    deep = ops.label_logprobs(dx.view(2, 3, 2, 37), labels.view(2, 3, 2), top=3, lse=True)
     for a, b in zip(flat, deep):
         assert b.shape[:3] == (2, 3, 2) and torch.equal(a.reshape(-1), b.reshape(-1))
-    one = ops.label_logprobs(dx[0], labels[0], top=3)
+    one = ops.label_logprobs(dx[0], labels[0], top=3, lse=True)
     assert one.logprob.shape == () and one.top_index.shape == (3,) and torch.equal(one.top_index, flat.top_index[0])
-    none = ops.label_logprobs(dx[:0], labels[:0], top=3)
+    none = ops.label_logprobs(dx[:0], labels[:0], top=3, lse=True)
     assert none.logprob.shape == (0,) and none.top_index.shape == (0, 3)
-    turned = ops.label_logprobs(dx.t().contiguous().t(), labels, top=3)  # (classes are not the innermost dimension)
-    same = ops.label_logprobs(dx[:1].expand(5, 37), labels[:1].expand(5), top=3)  # (rows of stride 0)
+    turned = ops.label_logprobs(dx.t().contiguous().t(), labels, top=3, lse=True)  # (classes are not the innermost dimension)
+    same = ops.label_logprobs(dx[:1].expand(5, 37), labels[:1].expand(5), top=3, lse=True)  # (rows of stride 0)
     for a, b, c in zip(flat, turned, same):
         assert torch.equal(a, b) and torch.equal(c, a[:1].expand_as(c))
 
@@ -152,7 +154,7 @@ def test_readout_of_odd_rows(classes, dtype):
     labels = torch.full((len(ROWS),), classes // 3)
     for top in {1, min(classes, 5), min(classes, 64)}:
         for temperature in (1.0, 2.0):
-            got = ops.label_logprobs(x.to(DEV), labels.to(DEV), top=top, temperature=temperature)
+            got = ops.label_logprobs(x.to(DEV), labels.to(DEV), top=top, lse=True, temperature=temperature)
             _check_readout(got, x, labels, top, temperature)
 
 
@@ -187,7 +189,7 @@ def test_readout_gradient(rows, classes, top, dtype):
         labels[rows // 2] = -100
         up = [torch.randn(rows, generator=gen) for _ in range(3)] + [torch.randn(rows, top, generator=gen)]
         leaf = dx.detach().requires_grad_()
-        o = ops.label_logprobs(leaf, labels.to(DEV), top=top, temperature=temperature)
+        o = ops.label_logprobs(leaf, labels.to(DEV), top=top, lse=True, temperature=temperature)
         for use in ((0,), (1,), (0, 1), (0, 1, 2, 3), (3,)):
             outs, ups = zip(*[((o.logprob, o.entropy, o.lse, o.top_logprob)[i], up[i].to(DEV)) for i in use])
             (grad,) = torch.autograd.grad(outs, leaf, ups, retain_graph=True)
@@ -382,7 +384,7 @@ def test_far_offsets():
     dx.copy_(x.to(DEV))
     labels = torch.tensor([1, 5000, 77])
     leaf = dx.detach().requires_grad_()
-    o = ops.label_logprobs(leaf, labels.to(DEV), top=8)
+    o = ops.label_logprobs(leaf, labels.to(DEV), top=8, lse=True)
     _check_readout(o, x, labels, 8, 1.0)
     (grad,) = torch.autograd.grad(o.logprob, leaf, torch.ones(3, device=DEV))
     want, bound = O.readout_grad(x, labels, 0, 1.0, torch.ones(3))
@@ -391,7 +393,7 @@ def test_far_offsets():
     rows = 70001
     big = torch.empty(rows, 32771, dtype=torch.bfloat16, device=DEV).normal_()
     leaf = big.requires_grad_()
-    o = ops.label_logprobs(leaf, top=2)
+    o = ops.label_logprobs(leaf, top=2, lse=True)
     (grad,) = torch.autograd.grad(o.entropy, leaf, torch.ones(rows, device=DEV))
     for r in (0, 40000, 65535, 65536, rows - 1):
         x = big[r:r + 1].detach().cpu()
@@ -411,7 +413,7 @@ def test_repeats_streams_and_graphs(rows, classes):
 
     def step(x):
         x = x.detach().requires_grad_()
-        o = ops.label_logprobs(x, labels, top=12)
+        o = ops.label_logprobs(x, labels, top=12, lse=True)
         g = torch.autograd.grad((o.logprob, o.entropy, o.top_logprob), x, (up, up, up[:, None].expand(rows, 12)))
         loss = ops.top_distill(x, index, value, tail=True)
         return [t.detach() for t in o] + [g[0], loss.detach(), torch.autograd.grad(loss, x, up)[0]]
@@ -463,6 +465,8 @@ def test_refusals():
             ops.label_logprobs(dx, labels, temperature=bad)
         with pytest.raises(ValueError, match="temperature"):
             ops.top_distill(dx, labels[:, None], dx[:, :1], temperature=bad)
+    with pytest.raises(ValueError, match="nothing"):
+        ops.label_logprobs(dx, entropy=False)
     with pytest.raises(ValueError, match="labels"):
         ops.label_logprobs(dx, labels[:3])
     with pytest.raises(_lib.VittaHipError, match="labels"):

@@ -6,6 +6,7 @@ is no eager fallback for the HIP path.
 """
 import ctypes as C
 import os
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -157,13 +158,31 @@ class LabelLogprobs(NamedTuple):
     """What `label_logprobs` answers; None for what was not asked."""
     logprob: Optional[torch.Tensor]
     entropy: Optional[torch.Tensor]
-    lse: torch.Tensor
+    lse: Optional[torch.Tensor]
     top_logprob: Optional[torch.Tensor]
     top_index: Optional[torch.Tensor]
 
 
+# These calls are short (a batch of class scores is a few microseconds of GPU time), so their host side is kept lean: plain integers to
+# ctypes, the raw stream, a device switch only where the tensors are not on the current device.
+def _call(name, device, *args):
+    """check(name(*args, stream)) on the tensors' device and its current stream."""
+    fn = getattr(lib(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    check(status, name)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _score_rows(x, name, temperature):
-    """(rows of the scores as a matrix whose last stride is 1, leading shape, classes, row stride); copies only what has no such view."""
+    """The scores as a matrix whose last stride is 1 (a view; a copy only of what has no such view)."""
     if not x.is_cuda:
         raise _lib.VittaHipError(f"{name} must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
     if x.dtype not in _SCORE_TYPES:
@@ -173,9 +192,7 @@ def _score_rows(x, name, temperature):
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"temperature must be a positive finite number (got {temperature})")
     m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if m.stride(1) != 1 or m.stride(0) < 0:
-        m = m.contiguous()
-    return m, x.shape[:-1], m.shape[1], m.stride(0)
+    return m if m.stride(1) == 1 else m.contiguous()
 
 
 def _score_side(t, name, like, shape, dtypes):
@@ -189,8 +206,13 @@ def _score_side(t, name, like, shape, dtypes):
     return (t.long() if t.dtype == torch.int32 else t).contiguous()
 
 
+@lru_cache(maxsize=4096)
+def _score_workspace_bytes(rows, classes, dtype, top):
+    return int(lib().vitta_scores_workspace_bytes(rows, classes, dtype, top))
+
+
 def _score_workspace(m, rows, classes, top):
-    n = int(lib().vitta_scores_workspace_bytes(rows, classes, _SCORE_TYPES[m.dtype], top))
+    n = _score_workspace_bytes(rows, classes, _SCORE_TYPES[m.dtype], top)
     return (torch.empty(n, dtype=torch.uint8, device=m.device) if n else None), n
 
 
@@ -198,116 +220,123 @@ def _row_gradient(g, rows):
     """(tensor or None, stride) of an upstream gradient per row; one value for every row (what mean() and sum() send) is not spread out."""
     if g is None:
         return None, 0
-    if rows > 1 and all(s == 0 or n == 1 for s, n in zip(g.stride(), g.shape)):
+    if g.is_contiguous():
+        return g, 1
+    if all(s == 0 or n == 1 for s, n in zip(g.stride(), g.shape)):
         return g, 0
     return g.contiguous(), 1
 
 
-def _label_logprobs(m, lead, labels, top, entropy, temperature, ignore_index, stats):
+def _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_index, stats):
     rows, classes = m.shape
-    f = dict(dtype=torch.float32, device=m.device)
-    logprob = torch.empty(lead, **f) if labels is not None else None
-    ent = torch.empty(lead, **f) if entropy else None
-    lse = torch.empty(lead, **f)
-    top_logprob = torch.empty(*lead, top, **f) if top else None
-    top_index = torch.empty(*lead, top, dtype=torch.int64, device=m.device) if top else None
+    device, f32 = m.device, torch.float32
+    logprob = torch.empty(lead, dtype=f32, device=device) if labels is not None else None
+    ent = torch.empty(lead, dtype=f32, device=device) if entropy else None
+    lse = torch.empty(lead, dtype=f32, device=device) if lse else None
+    top_logprob = torch.empty(*lead, top, dtype=f32, device=device) if top else None
+    top_index = torch.empty(*lead, top, dtype=torch.int64, device=device) if top else None
     if rows:
-        with torch.cuda.device(m.device):
-            ws, n = _score_workspace(m, rows, classes, top)
-            check(lib().vitta_label_logprobs_fwd(_p(m), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _p(labels),
-                                                 ignore_index, top, _p(logprob), _p(ent), _p(lse), _p(top_logprob), _p(top_index),
-                                                 _p(stats), _p(ws), n, _stream()), "vitta_label_logprobs_fwd")
+        ws, n = _score_workspace(m, rows, classes, top)
+        _call("vitta_label_logprobs_fwd", device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _ptr(labels),
+              ignore_index, top, _ptr(logprob), _ptr(ent), _ptr(lse), _ptr(top_logprob), _ptr(top_index), _ptr(stats), _ptr(ws), n)
     return logprob, ent, lse, top_logprob, top_index
 
 
 class _LabelLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, labels, top, entropy, temperature, ignore_index):
-        m, lead, _, _ = _score_rows(x, "logits", temperature)
+    def forward(ctx, m, lead, labels, top, entropy, lse, temperature, ignore_index):
         stats = torch.empty(m.shape[0], 4, dtype=torch.float32, device=m.device)
-        out = _label_logprobs(m, lead, labels, top, entropy, temperature, ignore_index, stats)
+        out = _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_index, stats)
         ctx.save_for_backward(m, labels, out[4], stats)
-        ctx.how = (x.shape, top, temperature, ignore_index)
+        ctx.how = (top, temperature, ignore_index)
         if top:
             ctx.mark_non_differentiable(out[4])
         ctx.set_materialize_grads(False)
         return out
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g_logprob, g_entropy, g_lse, g_top, _):
-        m, labels, top_index, stats = ctx.saved_tensors
-        shape, top, temperature, ignore_index = ctx.how
-        rows, classes = m.shape
-        dx = torch.empty(shape, dtype=m.dtype, device=m.device)
-        if rows:
-            (a, sa), (b, sb), (c, sc) = _row_gradient(g_logprob, rows), _row_gradient(g_entropy, rows), _row_gradient(g_lse, rows)
-            g_top = g_top.contiguous() if g_top is not None else None
-            with torch.cuda.device(m.device):
-                check(lib().vitta_label_logprobs_bwd(_p(m), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _p(labels),
-                                                     ignore_index, top, _p(top_index), _p(stats), _p(a), sa, _p(b), sb, _p(c), sc,
-                                                     _p(g_top), _p(dx), _stream()), "vitta_label_logprobs_bwd")
-        return dx, None, None, None, None, None
+    def backward(ctx, *g):
+        return (_label_logprobs_again if torch.is_grad_enabled() else _label_logprobs_grad)(ctx, *g)
 
 
-def label_logprobs(logits, labels=None, *, top=0, entropy=True, temperature=1.0, ignore_index=-100):
+def _label_logprobs_grad(ctx, g_logprob, g_entropy, g_lse, g_top, _):
+    m, labels, top_index, stats = ctx.saved_tensors
+    top, temperature, ignore_index = ctx.how
+    rows, classes = m.shape
+    dx = torch.empty(m.shape, dtype=m.dtype, device=m.device)
+    if rows:
+        (a, sa), (b, sb), (c, sc) = _row_gradient(g_logprob, rows), _row_gradient(g_entropy, rows), _row_gradient(g_lse, rows)
+        g_top = g_top.contiguous() if g_top is not None else None
+        _call("vitta_label_logprobs_bwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _ptr(labels),
+              ignore_index, top, _ptr(top_index), stats.data_ptr(), _ptr(a), sa, _ptr(b), sb, _ptr(c), sc, _ptr(g_top), dx.data_ptr())
+    return dx, None, None, None, None, None, None, None
+
+
+_label_logprobs_again = once_differentiable(_label_logprobs_grad)  # (under create_graph: a second derivative is refused, not taken as 0)
+
+
+def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, temperature=1.0, ignore_index=-100):
     """Log probability of given labels, entropy and best alternatives of rows of class scores, read once.
 
     logits (..., V) float32 / bfloat16 / float16 (rows may be cut from a wider matrix); labels (...) int64 or int32, or None.
     Returns a LabelLogprobs of float32 tensors shaped (...): with z = logits / temperature,
-      logprob       z[label] - lse; 0 where label == ignore_index; NaN where the label is no class
+      logprob       z[label] - lse; 0 where label == ignore_index; NaN where the label is no class (None without labels)
       entropy       -sum p log p, p = softmax(z) (None with entropy=False)
-      lse           log sum exp z
+      lse           log sum exp z (None unless lse=True)
       top_logprob, top_index (..., top): the `top` (at most 64) best classes in falling order, ties to the lowest index; index -1 and
                     log probability -inf where fewer classes have a score above -inf.
     A row of -inf only has log probabilities -inf, entropy 0 and gradient 0; a row with NaN or +inf answers NaN and -1.
     Differentiable once in logits through logprob, entropy, lse and top_logprob; the gradient has the logits' type."""
-    _score_rows(logits, "logits", temperature)
-    if not 0 <= top <= min(_lib.SCORES_MAX_TOP, logits.shape[-1]):
-        raise ValueError(f"top must be between 0 and min({_lib.SCORES_MAX_TOP}, classes = {logits.shape[-1]}) (got {top})")
+    m = _score_rows(logits, "logits", temperature)
+    if not 0 <= top <= min(_lib.SCORES_MAX_TOP, m.shape[1]):
+        raise ValueError(f"top must be between 0 and min({_lib.SCORES_MAX_TOP}, classes = {m.shape[1]}) (got {top})")
+    if labels is None and not (top or entropy or lse):
+        raise ValueError("nothing is asked: give labels, top, entropy or lse")
+    lead = logits.shape[:-1]
     if labels is not None:
-        labels = _score_side(labels, "labels", logits, logits.shape[:-1], (torch.int64, torch.int32))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return LabelLogprobs(*_LabelLogprobs.apply(logits, labels, int(top), bool(entropy), float(temperature), int(ignore_index)))
-    m, lead, _, _ = _score_rows(logits, "logits", temperature)
-    return LabelLogprobs(*_label_logprobs(m, lead, labels, int(top), entropy, float(temperature), int(ignore_index), None))
+        labels = _score_side(labels, "labels", logits, lead, (torch.int64, torch.int32))
+    if m.requires_grad and torch.is_grad_enabled():
+        return LabelLogprobs(*_LabelLogprobs.apply(m, lead, labels, int(top), entropy, lse, float(temperature), int(ignore_index)))
+    return LabelLogprobs(*_label_logprobs(m, lead, labels, int(top), entropy, lse, float(temperature), int(ignore_index), None))
 
 
 def _top_distill(m, lead, index, value, temperature, tail):
     rows, classes = m.shape
-    f = dict(dtype=torch.float32, device=m.device)
-    loss, stats, q = torch.empty(lead, **f), torch.empty(rows, 4, **f), torch.empty(index.shape, **f)
+    device, f32 = m.device, torch.float32
+    loss, stats, q = torch.empty(lead, dtype=f32, device=device), torch.empty(rows, 4, dtype=f32, device=device), \
+        torch.empty(index.shape, dtype=f32, device=device)
     if rows:
-        with torch.cuda.device(m.device):
-            ws, n = _score_workspace(m, rows, classes, 0)
-            check(lib().vitta_top_distill_fwd(_p(m), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _p(index), _p(value),
-                                              _SCORE_TYPES[value.dtype], index.shape[-1], int(tail), _p(loss), _p(stats), _p(q), _p(ws), n,
-                                              _stream()), "vitta_top_distill_fwd")
+        ws, n = _score_workspace(m, rows, classes, 0)
+        _call("vitta_top_distill_fwd", device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, index.data_ptr(),
+              value.data_ptr(), _SCORE_TYPES[value.dtype], index.shape[-1], tail, loss.data_ptr(), stats.data_ptr(), q.data_ptr(), _ptr(ws), n)
     return loss, stats, q
 
 
 class _TopDistill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, index, value, temperature, tail):
-        m, lead, _, _ = _score_rows(x, "student_logits", temperature)
+    def forward(ctx, m, lead, index, value, temperature, tail):
         loss, stats, q = _top_distill(m, lead, index, value, temperature, tail)
         ctx.save_for_backward(m, index, stats, q)
-        ctx.how = (x.shape, temperature)
+        ctx.temperature = temperature
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        m, index, stats, q = ctx.saved_tensors
-        shape, temperature = ctx.how
-        rows, classes = m.shape
-        dx = torch.empty(shape, dtype=m.dtype, device=m.device)
-        if rows:
-            g, sg = _row_gradient(g, rows)
-            with torch.cuda.device(m.device):
-                check(lib().vitta_top_distill_bwd(_p(m), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _p(index),
-                                                  index.shape[-1], _p(stats), _p(q), _p(g), sg, _p(dx), _stream()), "vitta_top_distill_bwd")
-        return dx, None, None, None, None
+        return (_top_distill_again if torch.is_grad_enabled() else _top_distill_grad)(ctx, g)
+
+
+def _top_distill_grad(ctx, g):
+    m, index, stats, q = ctx.saved_tensors
+    rows, classes = m.shape
+    dx = torch.empty(m.shape, dtype=m.dtype, device=m.device)
+    if rows:
+        g, sg = _row_gradient(g, rows)
+        _call("vitta_top_distill_bwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), ctx.temperature,
+              index.data_ptr(), index.shape[-1], stats.data_ptr(), q.data_ptr(), g.data_ptr(), sg, dx.data_ptr())
+    return dx, None, None, None, None, None
+
+
+_top_distill_again = once_differentiable(_top_distill_grad)
 
 
 def top_distill(student_logits, teacher_index, teacher_value, *, temperature=1.0, tail=False):
@@ -321,18 +350,18 @@ def top_distill(student_logits, teacher_index, teacher_value, *, temperature=1.0
                   student gives the classes outside the list (left out where that is nothing).
     A class listed twice counts with the sum of its probabilities.  No factor temperature ** 2 is applied.  Differentiable once in
     student_logits; the gradient has their type."""
-    _score_rows(student_logits, "student_logits", temperature)
+    m = _score_rows(student_logits, "student_logits", temperature)
     if teacher_index.dim() == 0 or not 1 <= teacher_index.shape[-1] <= _lib.SCORES_MAX_LIST:
         raise ValueError(f"teacher_index must hold 1 to {_lib.SCORES_MAX_LIST} classes per row (got shape {tuple(teacher_index.shape)})")
     if teacher_value.requires_grad:
         raise ValueError("teacher_value gets no gradient: detach it")
-    shape = student_logits.shape[:-1] + teacher_index.shape[-1:]
+    lead = student_logits.shape[:-1]
+    shape = lead + teacher_index.shape[-1:]
     index = _score_side(teacher_index, "teacher_index", student_logits, shape, (torch.int64, torch.int32))
-    value = _score_side(teacher_value, "teacher_value", student_logits, shape, tuple(_SCORE_TYPES))
-    if torch.is_grad_enabled() and student_logits.requires_grad:
-        return _TopDistill.apply(student_logits, index, value, float(temperature), bool(tail))
-    m, lead, _, _ = _score_rows(student_logits, "student_logits", temperature)
-    return _top_distill(m, lead, index, value, float(temperature), tail)[0]
+    value = _score_side(teacher_value, "teacher_value", student_logits, shape, _SCORE_TYPES)
+    if m.requires_grad and torch.is_grad_enabled():
+        return _TopDistill.apply(m, lead, index, value, float(temperature), bool(tail))
+    return _top_distill(m, lead, index, value, float(temperature), bool(tail))[0]
 
 
 # ------------------------------------------------------------------------------------------------
