@@ -30,7 +30,7 @@ constexpr float kLowest = -3.402823466e+38f;
 constexpr int kU = 4;              // 16-byte loads of a lane that are consumed together
 constexpr int kWaves = 8;          // waves of a workgroup that share a long row
 constexpr int kWaveRow = 4096;     // classes up to which a row belongs to one wave
-constexpr int kBuf = 64 + 8 * 64;  // candidates of a wave: 63 waiting and a whole vector of every lane
+constexpr int kKeys = 256;         // candidates that a wave keeps: 2 KiB of LDS
 constexpr int kMaxSegments = 64;
 constexpr int kTailSegment = 1 << 18;  // classes whose membership bits fit 32 KiB
 
@@ -121,74 +121,107 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t j) { return ((uint64_t)ordered(x + 0.f) << 32) | (uint32_t)~j; }  // (-0 becomes +0)
 __device__ __forceinline__ float value_of(uint64_t key) { return unordered((uint32_t)(key >> 32)); }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) { return __shfl_xor((unsigned long long)v, d); }
+
+// the value of lane ^ D: within a row of 16 by DPP, across rows by the swaps (a shuffle through LDS costs several times as much)
+template <int CTRL, int BANKS> __device__ __forceinline__ int dpp(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, 0xf, BANKS, false); }
+template <int D> __device__ __forceinline__ uint32_t lane_xor(uint32_t x, int lane) {
+  const int v = (int)x;
+  if (D == 1) return dpp<0xb1, 0xf>(v, v);                     // quad_perm 1 0 3 2
+  if (D == 2) return dpp<0x4e, 0xf>(v, v);                     // quad_perm 2 3 0 1
+  if (D == 4) return dpp<0x114, 0xa>(dpp<0x104, 0x5>(v, v), v);  // row_shl:4 into the even quads, row_shr:4 into the odd ones
+  if (D == 8) return dpp<0x128, 0xf>(v, v);                    // row_ror:8
+  if (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return (lane & 16) ? r[0] : r[1];
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return (lane & 32) ? r[0] : r[1];
+}
+template <int D> __device__ __forceinline__ uint64_t lane_xor(uint64_t v, int lane) {
+  return ((uint64_t)lane_xor<D>((uint32_t)(v >> 32), lane) << 32) | lane_xor<D>((uint32_t)v, lane);
+}
 
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
   __builtin_amdgcn_wave_barrier();
 }
 
-// a lower bound, good to 16 bits, of the r-th largest of the lanes' values: bit by bit, by counting lanes
-__device__ __forceinline__ float rth_largest(float v, int r) {
-  const uint32_t o = ordered(v);
-  uint32_t t = 0;
+// a lower bound, good to 16 bits, of the r-th largest of the lanes' M values: bit by bit, by counting
+template <int M> __device__ __forceinline__ float rth_largest(const float* v, int r) {
+  uint32_t o[M], t = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) o[i] = ordered(v[i]);
 #pragma unroll
   for (int b = 31; b >= 16; --b) {
     const uint32_t u = t | (1u << b);
-    if (__popcll(__ballot(o >= u)) >= r) t = u;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) n += __popcll(__ballot(o[i] >= u));
+    if (n >= r) t = u;
   }
   return t <= ordered(kLowest) ? kLowest : unordered(t);
 }
 
-// 64 keys across the lanes, falling
-__device__ __forceinline__ uint64_t sort64(uint64_t v, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-    for (int j = k >> 1; j >= 1; j >>= 1) {
-      const uint64_t o = shfl_xor64(v, j);
-      const bool keep_max = ((lane & j) == 0) == ((lane & k) == 0);
-      v = (o > v) == keep_max ? o : v;
-    }
-  return v;
+// one exchange of a bitonic network: the lane keeps the larger key where its bit D equals its bit K (K = 64: none has it), or the smaller
+template <int D, int K, bool RISING> __device__ __forceinline__ uint64_t exchange(uint64_t v, int lane) {
+  const uint64_t o = lane_xor<D>(v, lane);
+  const bool larger = (((lane & D) == 0) == ((lane & K) == 0)) != RISING;
+  return (o > v) == larger ? o : v;
 }
-// the 64 best of two falling lists
-__device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b, int lane) {
-  const uint64_t r = __shfl((unsigned long long)b, 63 - lane);
-  uint64_t v = a > r ? a : r;
-#pragma unroll
-  for (int j = 32; j >= 1; j >>= 1) {
-    const uint64_t o = shfl_xor64(v, j);
-    v = (o > v) == ((lane & j) == 0) ? o : v;
-  }
-  return v;
+template <int K, bool RISING> __device__ __forceinline__ uint64_t exchanges(uint64_t v, int lane) {
+  if (K >= 64) v = exchange<32, K, RISING>(v, lane);
+  if (K >= 32) v = exchange<16, K, RISING>(v, lane);
+  if (K >= 16) v = exchange<8, K, RISING>(v, lane);
+  if (K >= 8) v = exchange<4, K, RISING>(v, lane);
+  if (K >= 4) v = exchange<2, K, RISING>(v, lane);
+  return exchange<1, K, RISING>(v, lane);
+}
+// 64 keys across the lanes, rising
+__device__ __forceinline__ uint64_t sort64_rising(uint64_t v, int lane) {
+  v = exchanges<2, true>(v, lane);
+  v = exchanges<4, true>(v, lane);
+  v = exchanges<8, true>(v, lane);
+  v = exchanges<16, true>(v, lane);
+  v = exchanges<32, true>(v, lane);
+  return exchanges<64, true>(v, lane);
+}
+// the 64 best of a falling and a rising list, falling
+__device__ __forceinline__ uint64_t merge64(uint64_t falling, uint64_t rising, int lane) {
+  return exchanges<64, false>(falling > rising ? falling : rising, lane);
 }
 
 // a wave's list: lane i holds the i-th best key seen (0: none)
 struct Best {
   uint64_t mine;
-  uint64_t* buf;  // kBuf candidates in LDS
-  float bound;    // scores below it are not among the k best of the row
-  int waiting, k;
 
-  __device__ __forceinline__ void offer(float f, uint32_t j) {
-    const bool in = f >= bound;  // (false for NaN and -inf: the bound is finite)
-    const uint64_t who = __ballot(in);
-    if (who == 0) return;
-    if (in) buf[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key_of(f, j);
-    waiting += __popcll(who);
-  }
-  __device__ void take(int n, int lane) {  // the last n <= 64 waiting
-    wave_fence();
-    waiting -= n;
-    const uint64_t v = sort64(lane < n ? buf[waiting + lane] : 0, lane);
-    wave_fence();
-    mine = merge64(mine, v, lane);
-    const uint32_t o = __builtin_amdgcn_readlane((uint32_t)(mine >> 32), k - 1);
-    if (o) bound = fmaxf(bound, unordered(o));
-  }
-  __device__ __forceinline__ void settle(int lane) {
-    while (waiting >= 64) take(64, lane);
+  __device__ __forceinline__ void take(uint64_t key, int lane) { mine = merge64(mine, sort64_rising(key, lane), lane); }
+
+  // every score of a row that the wave's lanes have, for rows of which the bound lets too many pass (scores that rise along the row, or many
+  // equal ones): those from the list's k-th on wait in `buf` and are taken by 64.  all(e, &f): the lane's e-th class, and its score
+  template <class All> __device__ void take_all(int n, int k, uint64_t* buf, All all, int lane) {
+    int waiting = 0;
+    float bound = kLowest;
+    mine = 0;
+    for (int e = 0; e <= n; ++e) {
+      if (e < n) {
+        float f;
+        const uint32_t j = all(e, f);
+        const bool in = f >= bound;  // (false for NaN and -inf: the bound is finite)
+        const uint64_t who = __ballot(in);
+        if (who == 0) continue;
+        if (in) buf[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key_of(f, j);
+        waiting += __popcll(who);
+        wave_fence();
+      }
+      while (waiting >= 64 || (e == n && waiting > 0)) {
+        const int m = min(waiting, 64);
+        waiting -= m;
+        take(lane < m ? buf[waiting + lane] : 0, lane);
+        const uint32_t o = __builtin_amdgcn_readlane((uint32_t)(mine >> 32), k - 1);
+        if (o) bound = fmaxf(bound, unordered(o));
+        wave_fence();
+      }
+    }
   }
 };
 
@@ -336,7 +369,8 @@ template <typename T, int NW, int MODE, bool ENT, bool TOP>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdArgs A) {
   constexpr int N = Pack<T>::N, NT = NW * 64, G = NW == 1 ? 4 : 1;  // G groups in a workgroup
   extern __shared__ __attribute__((aligned(16))) uint32_t bits_all[];  // kDistillTail: one bit per class of the group's segment
-  __shared__ uint64_t buf[TOP ? (NW == 1 ? 4 : NW) * kBuf : 1];
+  __shared__ uint64_t keys_all[TOP ? (NW == 1 ? G : NW) * kKeys : 1];  // the waves' candidates, later their lists
+  __shared__ int counts[NW];
   __shared__ Sum red[NW];
   __shared__ float bounds[NW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = NW == 1 ? lane : threadIdx.x;
@@ -372,15 +406,27 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
   }
 
   Sum v{kLowest, 0.f, 0.f};
-  Best best{0, buf + (TOP ? wave * kBuf : 0), kLowest, 0, A.top};
   const float c = A.c;
+  float bound = kLowest;  // a lower bound of the row's top-th score
+  uint64_t* keys = keys_all + (TOP ? wave * kKeys : 0);
+  int waiting = 0;        // candidates found; beyond kKeys: not all of them are kept
+  auto offer = [&](float f, int j) {
+    const bool in = f >= bound;  // (never for NaN and -inf: the bound is finite)
+    const uint64_t who = __ballot(in);
+    if (who == 0) return;
+    const int many = __popcll(who);
+    if (in && waiting + many <= kKeys)
+      keys[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key_of(f, (uint32_t)(j0 + j));
+    waiting += many;
+  };
 
   // the vectors at + u * NT of this lane (those from nv on are empty)
   auto load = [&](uint4* w, int at) {
 #pragma unroll
     for (int u = 0; u < kU; ++u) w[u] = at + u * NT < nv ? xv[at + u * NT] : Pack<T>::empty();
   };
-  auto consume = [&](const uint4* w, int base, bool first) {
+  const int steps = max(1, (nv + kU * NT - 1) / (kU * NT));
+  auto consume = [&](const uint4* w, int base, int step) {
     float f[kU][N], cu[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -421,39 +467,43 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
       }
     }
     if (TOP) {
-      if (first) {  // every wave has r maxima at or above its bound: NW r >= k scores of the row are
-        best.bound = rth_largest(cm, (A.top + NW - 1) / NW);
+      // Each of the waves has r of its lanes' maxima at or above what it gives into `bounds`, so NW r >= top scores of the row lie at or
+      // above the least of these.  After the first step all wait for it; later, on steps 1, 2, 4, ..., the waves take what stands there.
+      const int r = (A.top + NW - 1) / NW;
+      if (step == 0) {
+        bound = r <= 16 ? rth_largest<1>(&cm, r) : rth_largest<kU>(cu, r);
         if (NW > 1) {
-          if (lane == 0) bounds[wave] = best.bound;
+          if (lane == 0) bounds[wave] = bound;
           __syncthreads();
-#pragma unroll
-          for (int o = 0; o < NW; ++o) best.bound = fminf(best.bound, bounds[o]);
         }
       }
-      if (__ballot(cm >= best.bound) != 0) {
-        uint32_t which = 0;
+      if (NW > 1) {
+        float least = __hip_atomic_load(&bounds[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 #pragma unroll
-        for (int u = 0; u < kU; ++u) which |= __ballot(cu[u] >= best.bound) != 0 ? 1u << u : 0u;
-        while (which) {
-          const int u = __builtin_ctz(which), at = base + u * NT + tid;
-          which &= which - 1;
-          float g[N];
-          Pack<T>::open(at < nv ? xv[at] : Pack<T>::empty(), g);  // (again: an index into registers has to be a constant)
+        for (int o = 1; o < NW; ++o) least = fminf(least, __hip_atomic_load(&bounds[o], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+        bound = least;
+      }
+      if (__ballot(cm >= bound) != 0) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) best.offer(g[i], (uint32_t)(j0 + head + at * N + i));
-          best.settle(lane);
+        for (int u = 0; u < kU; ++u) {
+          if (base + u * NT >= nv || __ballot(cu[u] >= bound) == 0) continue;
+#pragma unroll
+          for (int i = 0; i < N; ++i) offer(f[u][i], head + (base + u * NT + tid) * N + i);
         }
+      }
+      if (NW > 1 && step > 0 && (step & (step - 1)) == 0 && step + 1 < steps) {
+        const float mine = rth_largest<1>(&v.m, r);
+        if (lane == 0) __hip_atomic_store(&bounds[wave], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
     }
   };
 
   uint4 now[kU], next[kU];
   load(now, tid);
-  const int steps = max(1, (nv + kU * NT - 1) / (kU * NT));
   for (int step = 0; step < steps; ++step) {
     const int base = step * kU * NT;
     if (step + 1 < steps) load(next, base + kU * NT + tid);
-    consume(now, base, step == 0);
+    consume(now, base, step);
 #pragma unroll
     for (int u = 0; u < kU; ++u) now[u] = next[u];
   }
@@ -462,7 +512,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
     const int rest = n - nv * N, i = lane < head ? lane : body + lane - head;
     if (rest > 0) {
       float f = lane < rest ? to_float(x[i]) : -INFINITY;
-      if (TOP) best.offer(f, (uint32_t)(j0 + i));
+      if (TOP) offer(f, i);
       if (MODE == kDistillTail && lane < rest && (bits[(i - head + 16) >> 5] >> ((i - head + 16) & 31) & 1)) f = -INFINITY;
       v = moved(v, fmaxf(v.m, f), c);
       const float a = (f - v.m) * c, e = exp2_fast(a);
@@ -471,23 +521,51 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
     }
   }
   v = wave_merge(v, c);
-  if (TOP) {
-    best.settle(lane);
-    if (best.waiting) best.take(best.waiting, lane);
-  }
+  Best best{0};
   if (NW > 1) {
-    if (lane == 0) red[wave] = v;
-    if (TOP) best.buf[lane] = best.mine;
+    if (lane == 0) red[wave] = v, counts[wave] = waiting;
     __syncthreads();
-    if (TOP) {
+  } else {
+    wave_fence();
+  }
+  if (TOP) {
+    int most = waiting, before = 0, all = waiting;
+    if (NW > 1) {
+      all = most = 0;
+#pragma unroll
+      for (int o = 0; o < NW; ++o) most = max(most, counts[o]), all += counts[o];
+    }
+    if (most > kKeys) {
+      best.take_all((n + NT - 1) / NT, A.top, keys, [&](int e, float& f) {
+        const int j = e * NT + tid;
+        f = j < n ? to_float(x[j]) : -INFINITY;
+        return (uint32_t)(j0 + j);
+      }, lane);
+    } else if (NW > 1 && all <= 64) {  // one sort for all of them
+      uint64_t key = 0;
+#pragma unroll
+      for (int o = 0; o < NW; ++o) {
+        if (lane >= before && lane < before + counts[o]) key = keys_all[o * kKeys + lane - before];
+        before += counts[o];
+      }
+      if (wave == 0) best.take(key, lane);
+    } else {
+      for (int at = 0; at < waiting; at += 64) best.take(at + lane < waiting ? keys[at + lane] : 0, lane);
+    }
+    if (NW > 1 && (all > 64 || most > kKeys)) {  // the waves' lists, pair by pair
+      keys[lane] = best.mine;
+      __syncthreads();
+#pragma unroll
       for (int d = 1; d < NW; d <<= 1) {
         if ((wave & (2 * d - 1)) == 0) {
-          best.mine = merge64(best.mine, best.buf[d * kBuf + lane], lane);
-          best.buf[lane] = best.mine;
+          best.mine = merge64(best.mine, keys[d * kKeys + 63 - lane], lane);
+          keys[lane] = best.mine;
         }
         __syncthreads();
       }
     }
+  }
+  if (NW > 1) {
     if (wave != 0) return;
     v = lane < NW ? red[lane] : Sum{kLowest, 0.f, 0.f};
 #pragma unroll
@@ -514,7 +592,7 @@ __global__ __launch_bounds__(256) void scores_join_kernel(FwdArgs A) {
   uint64_t mine = 0;
   if (TOP) {
     for (int s = wave; s < A.segments; s += 4) {
-      const uint64_t o = lane < A.top ? A.keys[(row * A.segments + s) * A.top + lane] : 0;
+      const uint64_t o = 63 - lane < A.top ? A.keys[(row * A.segments + s) * A.top + 63 - lane] : 0;
       mine = merge64(mine, o, lane);
     }
     lists[threadIdx.x] = mine;
@@ -522,7 +600,7 @@ __global__ __launch_bounds__(256) void scores_join_kernel(FwdArgs A) {
   }
   if (wave != 0) return;
   if (TOP)
-    for (int w = 1; w < 4; ++w) mine = merge64(mine, lists[w * 64 + lane], lane);
+    for (int w = 1; w < 4; ++w) mine = merge64(mine, lists[w * 64 + 63 - lane], lane);
   Sum v{kLowest, 0.f, 0.f};
   if (lane < A.segments) {
     const float4 p = A.part[row * A.segments + lane];
