@@ -172,7 +172,7 @@ def _call(name, device, *args):
     if index == torch._C._cuda_getDevice():
         status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(device):  # (the library launches on the current device)
             status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     check(status, name)
 
@@ -213,7 +213,7 @@ def _score_workspace_bytes(rows, classes, dtype, top):
 
 def _score_workspace(m, rows, classes, top):
     n = _score_workspace_bytes(rows, classes, _SCORE_TYPES[m.dtype], top)
-    return (torch.empty(n, dtype=torch.uint8, device=m.device) if n else None), n
+    return (m.new_empty(n, dtype=torch.uint8) if n else None), n
 
 
 def _row_gradient(g, rows):
@@ -229,15 +229,15 @@ def _row_gradient(g, rows):
 
 def _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_index, stats):
     rows, classes = m.shape
-    device, f32 = m.device, torch.float32
-    logprob = torch.empty(lead, dtype=f32, device=device) if labels is not None else None
-    ent = torch.empty(lead, dtype=f32, device=device) if entropy else None
-    lse = torch.empty(lead, dtype=f32, device=device) if lse else None
-    top_logprob = torch.empty(*lead, top, dtype=f32, device=device) if top else None
-    top_index = torch.empty(*lead, top, dtype=torch.int64, device=device) if top else None
+    f32 = torch.float32
+    logprob = m.new_empty(lead, dtype=f32) if labels is not None else None
+    ent = m.new_empty(lead, dtype=f32) if entropy else None
+    lse = m.new_empty(lead, dtype=f32) if lse else None
+    top_logprob = m.new_empty((*lead, top), dtype=f32) if top else None
+    top_index = m.new_empty((*lead, top), dtype=torch.int64) if top else None
     if rows:
         ws, n = _score_workspace(m, rows, classes, top)
-        _call("vitta_label_logprobs_fwd", device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _ptr(labels),
+        _call("vitta_label_logprobs_fwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _ptr(labels),
               ignore_index, top, _ptr(logprob), _ptr(ent), _ptr(lse), _ptr(top_logprob), _ptr(top_index), _ptr(stats), _ptr(ws), n)
     return logprob, ent, lse, top_logprob, top_index
 
@@ -245,7 +245,7 @@ def _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_inde
 class _LabelLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, m, lead, labels, top, entropy, lse, temperature, ignore_index):
-        stats = torch.empty(m.shape[0], 4, dtype=torch.float32, device=m.device)
+        stats = m.new_empty((m.shape[0], 4), dtype=torch.float32)
         out = _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_index, stats)
         ctx.save_for_backward(m, labels, out[4], stats)
         ctx.how = (top, temperature, ignore_index)
@@ -263,7 +263,7 @@ def _label_logprobs_grad(ctx, g_logprob, g_entropy, g_lse, g_top, _):
     m, labels, top_index, stats = ctx.saved_tensors
     top, temperature, ignore_index = ctx.how
     rows, classes = m.shape
-    dx = torch.empty(m.shape, dtype=m.dtype, device=m.device)
+    dx = m.new_empty(m.shape)
     if rows:
         (a, sa), (b, sb), (c, sc) = _row_gradient(g_logprob, rows), _row_gradient(g_entropy, rows), _row_gradient(g_lse, rows)
         g_top = g_top.contiguous() if g_top is not None else None
@@ -302,21 +302,21 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
 
 def _top_distill(m, lead, index, value, temperature, tail):
     rows, classes = m.shape
-    device, f32 = m.device, torch.float32
-    loss, stats, q = torch.empty(lead, dtype=f32, device=device), torch.empty(rows, 4, dtype=f32, device=device), \
-        torch.empty(index.shape, dtype=f32, device=device)
+    k = index.shape[-1]
+    loss = m.new_empty(lead, dtype=torch.float32)
+    side = m.new_empty(rows * (4 + k), dtype=torch.float32)  # the row statistics (rows, 4), then the teacher's probabilities (rows, k)
     if rows:
         ws, n = _score_workspace(m, rows, classes, 0)
-        _call("vitta_top_distill_fwd", device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, index.data_ptr(),
-              value.data_ptr(), _SCORE_TYPES[value.dtype], index.shape[-1], tail, loss.data_ptr(), stats.data_ptr(), q.data_ptr(), _ptr(ws), n)
-    return loss, stats, q
+        _call("vitta_top_distill_fwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, index.data_ptr(),
+              value.data_ptr(), _SCORE_TYPES[value.dtype], k, tail, loss.data_ptr(), side.data_ptr(), side.data_ptr() + 16 * rows, _ptr(ws), n)
+    return loss, side
 
 
 class _TopDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, m, lead, index, value, temperature, tail):
-        loss, stats, q = _top_distill(m, lead, index, value, temperature, tail)
-        ctx.save_for_backward(m, index, stats, q)
+        loss, side = _top_distill(m, lead, index, value, temperature, tail)
+        ctx.save_for_backward(m, index, side)
         ctx.temperature = temperature
         return loss
 
@@ -326,13 +326,13 @@ class _TopDistill(torch.autograd.Function):
 
 
 def _top_distill_grad(ctx, g):
-    m, index, stats, q = ctx.saved_tensors
+    m, index, side = ctx.saved_tensors
     rows, classes = m.shape
-    dx = torch.empty(m.shape, dtype=m.dtype, device=m.device)
+    dx = m.new_empty(m.shape)
     if rows:
         g, sg = _row_gradient(g, rows)
         _call("vitta_top_distill_bwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), ctx.temperature,
-              index.data_ptr(), index.shape[-1], stats.data_ptr(), q.data_ptr(), g.data_ptr(), sg, dx.data_ptr())
+              index.data_ptr(), index.shape[-1], side.data_ptr(), side.data_ptr() + 16 * rows, g.data_ptr(), sg, dx.data_ptr())
     return dx, None, None, None, None, None
 
 
