@@ -28,7 +28,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLowest = -3.402823466e+38f;
 constexpr int kU = 4;              // 16-byte loads of a lane that are consumed together
-constexpr int kWaves = 8;          // waves of a workgroup that share a long row
+// Waves of a workgroup that share a long row: eight, four where it collects alternatives (2048 x 32003 float16: 27.0 us with eight and 29.5 with four
+// without alternatives, 40.3 and 36.5 with five of them; 4096 x 131072 bfloat16 with 64 of them 223 and 203).
+constexpr int waves_of(bool top) { return top ? 4 : 8; }
 constexpr int kWaveRow = 4096;     // classes up to which a row belongs to one wave
 constexpr int kKeys = 256;         // candidates that a wave keeps: 2 KiB of LDS
 constexpr int kMaxSegments = 64;
@@ -400,6 +402,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
   const int nv = (n - head) / N, body = head + nv * N;
   const uint4* xv = reinterpret_cast<const uint4*>(x + head);
 
+  // the vectors at + u * NT of this lane (those from nv on are empty)
+  auto load = [&](uint4* w, int at) {
+#pragma unroll
+    for (int u = 0; u < kU; ++u) w[u] = at + u * NT < nv ? load_once(xv + at + u * NT) : Pack<T>::empty();
+  };
+  uint4 now[kU], next[kU];
+  load(now, tid);
+
   uint32_t* bits = bits_all;
   if (MODE == kDistillTail) {  // class j0 + i at bit i - head + 16: a vector's bits never straddle a byte
     const int words = (A.per_segment + 16 + 31) / 32 + 1;
@@ -407,8 +417,10 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
     for (int i = tid; i < words; i += NT) bits[i] = 0;
     if (NW > 1) __syncthreads(); else wave_fence();
     for (int k = tid; k < A.list; k += NT) {
-      const int64_t j = A.index[row * A.list + k] - j0;
-      if (j >= 0 && j < n) atomicOr(&bits[(j - head + 16) >> 5], 1u << ((j - head + 16) & 31));
+      const int64_t j = A.index[row * A.list + k];
+      if (j < j0 || j >= j0 + (int64_t)n) continue;
+      const uint32_t bit = (uint32_t)(j - j0) - head + 16;
+      atomicOr(&bits[bit >> 5], 1u << (bit & 31));
     }
     if (NW > 1) __syncthreads(); else wave_fence();
   }
@@ -428,11 +440,6 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
     waiting += many;
   };
 
-  // the vectors at + u * NT of this lane (those from nv on are empty)
-  auto load = [&](uint4* w, int at) {
-#pragma unroll
-    for (int u = 0; u < kU; ++u) w[u] = at + u * NT < nv ? load_once(xv + at + u * NT) : Pack<T>::empty();
-  };
   const int steps = max(1, (nv + kU * NT - 1) / (kU * NT));
   auto consume = [&](const uint4* w, int base, int step) {
     float f[kU][N], cu[kU];
@@ -506,8 +513,6 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
     }
   };
 
-  uint4 now[kU], next[kU];
-  load(now, tid);
   for (int step = 0; step < steps; ++step) {
     const int base = step * kU * NT;
     if (step + 1 < steps) load(next, base + kU * NT + tid);
@@ -805,7 +810,8 @@ int launch_fwd(FwdArgs a, void* ws, hipStream_t st) {
     a.part = static_cast<float4*>(ws);
     a.keys = reinterpret_cast<uint64_t*>(a.part + a.rows * cut.segments);
   }
-  VITTA_LAUNCH((scores_kernel<T, kWaves, MODE, ENT, TOP>), dim3((unsigned)(a.rows * cut.segments)), dim3(kWaves * 64), bits, st, a);
+  constexpr int NW = waves_of(TOP);
+  VITTA_LAUNCH((scores_kernel<T, NW, MODE, ENT, TOP>), dim3((unsigned)(a.rows * cut.segments)), dim3(NW * 64), bits, st, a);
   if (cut.segments > 1) VITTA_LAUNCH((scores_join_kernel<T, MODE, TOP>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
   return VITTA_OK;
 }
