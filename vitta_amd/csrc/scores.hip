@@ -101,37 +101,7 @@ __device__ __forceinline__ float nan_f() { return __builtin_nanf(""); }
 // (x - m) / T; halved first, for two finite scores may lie further apart than a float reaches while this does not
 __device__ __forceinline__ float below(float x, float m, float inv_t) { return (0.5f * x - 0.5f * m) * (2.f * inv_t); }
 
-// ---- running sums ----------------------------------------------------------------------------------------------------------------
-// (max, sum of 2^a, sum of a 2^a); a is clamped where its power is 0 anyway, so that 0 * -inf never forms (a NaN reaches s unclamped)
-struct Sum {
-  float m, s, t;
-};
-__device__ __forceinline__ float clamped(float a) { return fmaxf(a, -200.f); }
-__device__ __forceinline__ Sum moved(Sum v, float m, float c) {
-  const float d = clamped((v.m - m) * c), r = exp2_fast(d);
-  return Sum{m, v.s * r, r * (v.t + v.s * d)};
-}
-__device__ __forceinline__ Sum merge(Sum a, Sum b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  a = moved(a, m, c), b = moved(b, m, c);
-  return Sum{m, a.s + b.s, a.t + b.t};
-}
-__device__ __forceinline__ Sum wave_merge(Sum v, float c) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = merge(v, Sum{__shfl_xor(v.m, d), __shfl_xor(v.s, d), __shfl_xor(v.t, d)}, c);
-  return v;
-}
-
-// ---- best alternatives -------------------------------------------------------------------------------------------------------------
-// orders scores by value, then by lowest class; 0 is below every finite score
-__device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
-}
-__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t j) { return ((uint64_t)ordered(x + 0.f) << 32) | (uint32_t)~j; }  // (-0 becomes +0)
-__device__ __forceinline__ float value_of(uint64_t key) { return unordered((uint32_t)(key >> 32)); }
-
+// ---- lanes ------------------------------------------------------------------------------------------------------------------------------
 // the value of lane ^ D: within a row of 16 by DPP, across rows by the swaps (a shuffle through LDS costs several times as much)
 template <int CTRL, int BANKS> __device__ __forceinline__ int dpp(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, 0xf, BANKS, false); }
 template <int D> __device__ __forceinline__ uint32_t lane_xor(uint32_t x, int lane) {
@@ -150,6 +120,42 @@ template <int D> __device__ __forceinline__ uint32_t lane_xor(uint32_t x, int la
 template <int D> __device__ __forceinline__ uint64_t lane_xor(uint64_t v, int lane) {
   return ((uint64_t)lane_xor<D>((uint32_t)(v >> 32), lane) << 32) | lane_xor<D>((uint32_t)v, lane);
 }
+
+template <class Op> __device__ __forceinline__ float wave_all(float v, int lane, Op op) {
+  v = op(v, __uint_as_float(lane_xor<1>(__float_as_uint(v), lane)));
+  v = op(v, __uint_as_float(lane_xor<2>(__float_as_uint(v), lane)));
+  v = op(v, __uint_as_float(lane_xor<4>(__float_as_uint(v), lane)));
+  v = op(v, __uint_as_float(lane_xor<8>(__float_as_uint(v), lane)));
+  v = op(v, __uint_as_float(lane_xor<16>(__float_as_uint(v), lane)));
+  return op(v, __uint_as_float(lane_xor<32>(__float_as_uint(v), lane)));
+}
+__device__ __forceinline__ float all_max(float v, int lane) { return wave_all(v, lane, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float all_sum(float v, int lane) { return wave_all(v, lane, [](float a, float b) { return a + b; }); }
+
+// ---- running sums ----------------------------------------------------------------------------------------------------------------
+// (max, sum of 2^a, sum of a 2^a); a is clamped where its power is 0 anyway, so that 0 * -inf never forms (a NaN reaches s unclamped)
+struct Sum {
+  float m, s, t;
+};
+__device__ __forceinline__ float clamped(float a) { return fmaxf(a, -200.f); }
+__device__ __forceinline__ Sum moved(Sum v, float m, float c) {
+  const float d = clamped((v.m - m) * c), r = exp2_fast(d);
+  return Sum{m, v.s * r, r * (v.t + v.s * d)};
+}
+__device__ __forceinline__ Sum wave_merge(Sum v, float c, int lane) {
+  v = moved(v, all_max(v.m, lane), c);
+  return Sum{v.m, all_sum(v.s, lane), all_sum(v.t, lane)};
+}
+
+// ---- best alternatives -------------------------------------------------------------------------------------------------------------
+// orders scores by value, then by lowest class; 0 is below every finite score
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu)); }
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t j) { return ((uint64_t)ordered(x + 0.f) << 32) | (uint32_t)~j; }  // (-0 becomes +0)
+__device__ __forceinline__ float value_of(uint64_t key) { return unordered((uint32_t)(key >> 32)); }
 
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
@@ -186,14 +192,15 @@ template <int K, bool RISING> __device__ __forceinline__ uint64_t exchanges(uint
   if (K >= 4) v = exchange<2, K, RISING>(v, lane);
   return exchange<1, K, RISING>(v, lane);
 }
-// 64 keys across the lanes, rising
-__device__ __forceinline__ uint64_t sort64_rising(uint64_t v, int lane) {
-  v = exchanges<2, true>(v, lane);
-  v = exchanges<4, true>(v, lane);
-  v = exchanges<8, true>(v, lane);
-  v = exchanges<16, true>(v, lane);
-  v = exchanges<32, true>(v, lane);
-  return exchanges<64, true>(v, lane);
+// n <= 64 keys in the first lanes (0 behind them), sorted; falling with n <= 32 leaves out the stages that only move zeros
+template <bool RISING> __device__ __forceinline__ uint64_t sort64(uint64_t v, int n, int lane) {
+  v = exchanges<2, RISING>(v, lane);
+  v = exchanges<4, RISING>(v, lane);
+  v = exchanges<8, RISING>(v, lane);
+  v = exchanges<16, RISING>(v, lane);
+  if (RISING || n > 16) v = exchanges<32, RISING>(v, lane);
+  if (RISING || n > 32) v = exchanges<64, RISING>(v, lane);
+  return v;
 }
 // the 64 best of a falling and a rising list, falling
 __device__ __forceinline__ uint64_t merge64(uint64_t falling, uint64_t rising, int lane) {
@@ -203,15 +210,18 @@ __device__ __forceinline__ uint64_t merge64(uint64_t falling, uint64_t rising, i
 // a wave's list: lane i holds the i-th best key seen (0: none)
 struct Best {
   uint64_t mine;
+  bool some;
 
-  __device__ __forceinline__ void take(uint64_t key, int lane) { mine = merge64(mine, sort64_rising(key, lane), lane); }
+  __device__ __forceinline__ void take(uint64_t key, int n, int lane) {  // n <= 64 keys in the first lanes, 0 behind them
+    mine = some ? merge64(mine, sort64<true>(key, n, lane), lane) : sort64<false>(key, n, lane);
+    some = true;
+  }
 
   // every score of a row that the wave's lanes have, for rows of which the bound lets too many pass (scores that rise along the row, or many
   // equal ones): those from the list's k-th on wait in `buf` and are taken by 64.  all(e, &f): the lane's e-th class, and its score
   template <class All> __device__ void take_all(int n, int k, uint64_t* buf, All all, int lane) {
     int waiting = 0;
     float bound = kLowest;
-    mine = 0;
     for (int e = 0; e <= n; ++e) {
       if (e < n) {
         float f;
@@ -226,7 +236,7 @@ struct Best {
       while (waiting >= 64 || (e == n && waiting > 0)) {
         const int m = min(waiting, 64);
         waiting -= m;
-        take(lane < m ? buf[waiting + lane] : 0, lane);
+        take(lane < m ? buf[waiting + lane] : 0, m, lane);
         const uint32_t o = __builtin_amdgcn_readlane((uint32_t)(mine >> 32), k - 1);
         if (o) bound = fmaxf(bound, unordered(o));
         wave_fence();
@@ -326,23 +336,23 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) m = fmaxf(m, z[i]);
-    m = wave_max(m);
+    m = all_max(m, lane);
     float in = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i)
       if (at[i] >= 0 && !(again >> i & 1)) in += exp2_fast((z[i] - m) * A.c);
     rest = v.s * exp2_fast((v.m - m) * A.c);
-    s = rest + wave_sum(in);
+    s = rest + all_sum(in, lane);
   }
   const float l2 = log2_fast(s);
-  const float ref = TAIL ? 0.f : wave_max(vm), cv = TAIL ? kLog2e : A.c;
+  const float ref = TAIL ? 0.f : all_max(vm, lane), cv = TAIL ? kLog2e : A.c;
   float q[R], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     q[i] = at[i] >= 0 ? exp2_fast((val[i] - ref) * cv) : 0.f;
     sum += q[i];
   }
-  sum = wave_sum(sum);
+  sum = all_sum(sum, lane);
   const float inv = TAIL ? 1.f : 1.f / sum, ql = TAIL ? 0.f : kLn2 * log2_fast(sum);
   float loss = 0.f;
 #pragma unroll
@@ -357,7 +367,7 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
     }
     if (k < K) A.q[row * K + k] = q[i];
   }
-  loss = wave_sum(loss);
+  loss = all_sum(loss, lane);
   if (lane != 0) return;
   float inside = !some ? 0.f : TAIL ? sum : 1.f, outside = inside;
   if (TAIL && some) {
@@ -486,7 +496,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
       // above the least of these.  After the first step all wait for it; later, on steps 1, 2, 4, ..., the waves take what stands there.
       const int r = (A.top + NW - 1) / NW;
       if (step == 0) {
-        bound = r <= 16 ? rth_largest<1>(&cm, r) : rth_largest<kU>(cu, r);
+        bound = r <= 32 ? rth_largest<1>(&cm, r) : rth_largest<kU>(cu, r);
         if (NW > 1) {
           if (lane == 0) bounds[wave] = bound;
           __syncthreads();
@@ -533,8 +543,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
       v.t = fmaf(e, clamped(a), v.t);
     }
   }
-  v = wave_merge(v, c);
-  Best best{0};
+  v = wave_merge(v, c, lane);
+  Best best{0, false};
   if (NW > 1) {
     if (lane == 0) red[wave] = v, counts[wave] = waiting;
     __syncthreads();
@@ -561,9 +571,9 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
         if (lane >= before && lane < before + counts[o]) key = keys_all[o * kKeys + lane - before];
         before += counts[o];
       }
-      if (wave == 0) best.take(key, lane);
+      if (wave == 0) best.take(key, all, lane);
     } else {
-      for (int at = 0; at < waiting; at += 64) best.take(at + lane < waiting ? keys[at + lane] : 0, lane);
+      for (int at = 0; at < waiting; at += 64) best.take(at + lane < waiting ? keys[at + lane] : 0, min(waiting - at, 64), lane);
     }
     if (NW > 1 && (all > 64 || most > kKeys)) {  // the waves' lists, pair by pair
       keys[lane] = best.mine;
@@ -581,9 +591,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
   if (NW > 1) {
     if (wave != 0) return;
     v = lane < NW ? red[lane] : Sum{kLowest, 0.f, 0.f};
-#pragma unroll
-    for (int d = NW / 2; d >= 1; d >>= 1) v = merge(v, Sum{__shfl_xor(v.m, d), __shfl_xor(v.s, d), __shfl_xor(v.t, d)}, c);
-    v.m = __shfl(v.m, 0), v.s = __shfl(v.s, 0), v.t = __shfl(v.t, 0);
+    v = wave_merge(v, c, lane);
     if (A.segments > 1) {
       const int64_t at = row * A.segments + seg;
       if (lane == 0) A.part[at] = make_float4(v.m, v.s, v.t, 0.f);
@@ -619,7 +627,7 @@ __global__ __launch_bounds__(256) void scores_join_kernel(FwdArgs A) {
     const float4 p = A.part[row * A.segments + lane];
     v = Sum{p.x, p.y, p.z};
   }
-  v = wave_merge(v, A.c);
+  v = wave_merge(v, A.c, lane);
   if (MODE == kReadout) finish_readout<T>(A, row, x, v, mine, lane);
   else finish_distill<T, MODE == kDistillTail>(A, row, x, v, lane);
 }
@@ -709,7 +717,7 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
       const int64_t j = valid ? A.top_index[row * A.top + lane] : -1;
       const float g = valid ? A.g_top[row * A.top + lane] : 0.f;
       if (tid < 64) collect(j, g * A.inv_t, j >= 0);
-      all -= wave_sum(j >= 0 ? g : 0.f);
+      all -= all_sum(j >= 0 ? g : 0.f, lane);
     }
     a0 = is * A.inv_t * (all + (ENT ? gh * kLn2 * st.z * is : 0.f));
     a1 = ENT ? -is * A.inv_t * gh * kLn2 : 0.f;
