@@ -158,6 +158,32 @@ def test_readout_of_odd_rows(classes, dtype):
             _check_readout(got, x, labels, top, temperature)
 
 
+@pytest.mark.parametrize("rows,classes", [(6, 4090), (4, 300001), (530, 20001)])
+@pytest.mark.parametrize("top", [1, 5, 64])
+def test_rows_that_hide_their_best(rows, classes, top):
+    """Rows whose first classes say nothing of the best ones: rising scores, a masked first part, equal scores, one plateau, late spikes."""
+    from vitta_amd import ops
+    gen = torch.Generator().manual_seed(classes)
+    x = torch.randn(rows, classes, generator=gen)
+    for r in range(rows):
+        kind = r % 6
+        if kind == 0:
+            x[r] = torch.arange(classes) * 1e-3
+        elif kind == 1:
+            x[r, : classes * 2 // 3] = -math.inf
+        elif kind == 2:
+            x[r] = 0.25
+        elif kind == 3:
+            x[r, classes // 2:] = 9.0
+        elif kind == 4:
+            x[r, -100:] += 20.0
+        else:
+            x[r] = torch.sort(x[r]).values
+    x = x.bfloat16() if rows < 100 else x
+    got = ops.label_logprobs(x.to(DEV), top=top)
+    _check_readout(got, x, None, top, 1.0)
+
+
 @pytest.mark.parametrize("classes", [101, 5000])
 def test_labels_that_are_no_class(classes):
     from vitta_amd import ops

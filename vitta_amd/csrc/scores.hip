@@ -508,6 +508,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
         for (int o = 1; o < NW; ++o) least = fminf(least, __hip_atomic_load(&bounds[o], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
         bound = least;
       }
+      // Where most lanes pass (masked classes came first, or scores rise along the row) the wave's own top-th maximum of this step is a bound too.
+      if (step > 0 && __popcll(__ballot(cm >= bound)) > 48) bound = fmaxf(bound, rth_largest<kU>(cu, A.top));
       if (__ballot(cm >= bound) != 0) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
