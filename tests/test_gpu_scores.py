@@ -379,6 +379,34 @@ def test_distillation_of_odd_rows(classes, tail):
     assert (padded == 0).all() and (torch.autograd.grad(padded.sum(), leaf)[0] == 0).all()
 
 
+@pytest.mark.parametrize("classes", [101, 5000])
+@pytest.mark.parametrize("gap", [60.0, 90.0, 140.0, 1000.0])
+def test_distillation_of_a_certain_student(classes, gap):
+    """A student that gives the classes outside the list next to nothing (their sum underflows 32 bits): their share of the rest holds."""
+    from vitta_amd import ops
+    dx, x = _scores(3, classes, torch.float32, 13)
+    index, value = _list(3, classes, 6, 7, True, ragged=False)
+    x.scatter_add_(1, index, torch.full((3, 6), gap))
+    leaf = x.to(DEV).requires_grad_()
+    loss = ops.top_distill(leaf, index.to(DEV), value.to(DEV), tail=True)
+    (grad,) = torch.autograd.grad(loss.sum(), leaf)
+    z = x.double()
+    listed = torch.zeros_like(z, dtype=torch.bool).scatter_(1, index, True)
+    rest = 1 - torch.exp(value.double()).sum(1)
+    lse = torch.logsumexp(z, 1)
+    lse_out = torch.logsumexp(torch.where(listed, -math.inf, z), 1)
+    want = (torch.exp(value.double()) * (value.double() - (z - lse[:, None]).gather(1, index))).sum(1) + rest * (torch.log(rest) - lse_out + lse)
+    # 8 u on each logarithm and on the differences of scores, (depth + 40) u on the sums, 8 u on the list's mass
+    scale = lse.abs() + lse_out.abs() + gap + value.double().abs().amax(1) + 2
+    _close(loss, want, O.U * (O.depth(classes) + 100) * scale, "loss")
+    share = torch.exp(torch.where(listed, -math.inf, z) - lse_out[:, None])
+    grad_want = torch.exp(z - lse[:, None]) - torch.zeros_like(z).scatter_(1, index, torch.exp(value.double())) - rest[:, None] * share
+    spread = (z.amax(1, keepdim=True) - z).abs()
+    bound = O.U * (O.depth(classes) + 60 + 8 * torch.where(listed, spread, spread - gap).abs()) * (torch.exp(z - lse[:, None]) + share) \
+        + 40 * O.U * (listed * 1.0 + share)
+    _check_grad(grad, grad_want, bound, torch.float32)
+
+
 def test_teacher_list_from_the_readout_trains_a_student():
     """The operators as they are used together: a teacher's readout gives the list, the student's loss and gradient follow, and the
     gradient points to the teacher (its step lowers the loss by the first order term)."""

@@ -95,6 +95,11 @@ __device__ __forceinline__ uint4 load_once(const uint4* p) {
   return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
+__device__ __forceinline__ void store_once(uint4* p, uint4 w) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store((u4){w.x, w.y, w.z, w.w}, reinterpret_cast<u4*>(p));
+}
+
 __device__ __forceinline__ float exp2_fast(float a) { return __builtin_amdgcn_exp2f(a); }
 __device__ __forceinline__ float log2_fast(float a) { return __builtin_amdgcn_logf(a); }
 __device__ __forceinline__ float nan_f() { return __builtin_nanf(""); }
@@ -369,18 +374,22 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
   }
   loss = all_sum(loss, lane);
   if (lane != 0) return;
-  float inside = !some ? 0.f : TAIL ? sum : 1.f, outside = inside;
+  // The gradient is e_j a - q_j: (m, a) of the listed classes, and of the others, whose e_j is taken against their own maximum: their share of
+  // the rest, q_rest e_j / sum e, then holds however little the student gives them.
+  const float inside = !some ? 0.f : TAIL ? sum : 1.f;
+  float4 st = make_float4(m, s == 0.f ? 0.f : inside / s, m, s == 0.f ? 0.f : inside / s);
   if (TAIL && some) {
     const float q_rest = fmaxf(1.f - sum, 0.f);
-    if (q_rest > 0.f && rest > 0.f) {
-      loss += q_rest * kLn2 * (log2_fast(q_rest) - log2_fast(rest / s));
-      inside = sum + q_rest;
-      outside = inside - q_rest * s / rest;
-    }
-    if (sum != sum || s != s) loss = nan_f();  // (comparisons with a NaN are false)
+    const bool both = q_rest > 0.f && v.s > 0.f;  // (of a NaN neither is true)
+    if (both) loss += q_rest * (kLn2 * (log2_fast(q_rest) + l2 - log2_fast(v.s)) - below(v.m, m, A.inv_t));
+    const float all = both ? sum + q_rest : sum;
+    st.y = s == 0.f ? 0.f : all / s;
+    st.z = v.m;
+    st.w = v.s == 0.f ? 0.f : all * (rest / s) / v.s - (both ? q_rest / v.s : 0.f);
+    if (sum != sum || s != s) loss = nan_f();
   }
   A.loss[row] = some ? loss : 0.f;
-  reinterpret_cast<float4*>(A.stats)[row] = make_float4(m, s, inside, outside);
+  reinterpret_cast<float4*>(A.stats)[row] = some ? st : make_float4(m, 0.f, m, 0.f);
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------------
@@ -652,6 +661,7 @@ struct BwdArgs {
   int32_t list;
   const float *q, *g;
   int64_t s_g;
+  int32_t stream_out;
 };
 
 // dx_j = e_j (a0 + a1 a_j), with a0 = at0 for the classes of the group's list, to which it adds `add`.
@@ -684,7 +694,7 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
   load(tid);
 
   const float4 st = reinterpret_cast<const float4*>(A.stats)[row];
-  const float m = st.x, is = st.y == 0.f ? 0.f : 1.f / st.y, c = A.c;
+  const float m = DISTILL ? st.z : st.x, is = st.y == 0.f ? 0.f : 1.f / st.y, c = A.c;  // (distillation: see finish_distill)
   float a0, a1 = 0.f, at0;
   int many = 0;  // the listed classes that lie here, in the list's order: the group's first wave collects them
   auto collect = [&](int64_t j, float value, bool valid) {
@@ -705,8 +715,8 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
         collect(valid ? A.index[row * A.list + k] : 0, valid ? -g * A.q[row * A.list + k] : 0.f, valid);
       }
     }
-    at0 = st.z == 0.f || g == 0.f ? 0.f : g * is * st.z;
-    a0 = st.w == 0.f || g == 0.f ? 0.f : g * is * st.w;
+    at0 = g == 0.f ? 0.f : g * st.y;
+    a0 = g == 0.f ? 0.f : g * st.w;
   } else {
     const int64_t y = A.g_logprob ? A.labels[row] : A.ignore;
     float gl = y != A.ignore ? A.g_logprob[row * A.s_logprob] : 0.f;
@@ -728,7 +738,7 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
   }
   if (tid == 0) many_all[group] = many;
   const bool dead = a0 == 0.f && a1 == 0.f;  // zeros whatever the row holds
-  auto grad = [&](float f, float b) {
+  auto grad = [&](float f, float m, float b) {
     const float a = (f - m) * c, e = exp2_fast(a);
     return e * (ENT ? fmaf(a1, clamped(a), b) : b);
   };
@@ -742,9 +752,10 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
         float f[N];
         Pack<T>::open(w[u], f);
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = dead ? 0.f : grad(f[e], a0);
+        for (int e = 0; e < N; ++e) f[e] = dead ? 0.f : grad(f[e], m, a0);
         const uint4 o = Pack<T>::close(f);
-        if (straight) reinterpret_cast<uint4*>(dx + head)[i] = o;
+        if (straight && A.stream_out) store_once(reinterpret_cast<uint4*>(dx + head) + i, o);
+        else if (straight) reinterpret_cast<uint4*>(dx + head)[i] = o;
         else __builtin_memcpy(__builtin_assume_aligned(dx + head + (int64_t)i * N, sizeof(T)), &o, 16);
       }
     }
@@ -754,7 +765,7 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
   }
   if (tid < n - nv * N) {
     const int i = tid < head ? tid : body + tid - head;
-    dx[i] = from_float<T>(dead ? 0.f : grad(to_float(x[i]), a0));
+    dx[i] = from_float<T>(dead ? 0.f : grad(to_float(x[i]), m, a0));
   }
   // the listed classes again, each with all that is added to it
   if (NT > 64) __syncthreads(); else wave_fence();
@@ -763,7 +774,7 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
     const int j = at[k];
     float sum = 0.f;
     for (int o = 0; o < many; ++o) sum += at[o] == j ? add[o] : 0.f;
-    dx[j] = from_float<T>((at0 == 0.f && a1 == 0.f ? 0.f : grad(to_float(x[j]), at0)) + sum);
+    dx[j] = from_float<T>((at0 == 0.f && a1 == 0.f ? 0.f : grad(to_float(x[j]), st.x, at0)) + sum);
   }
 }
 
@@ -839,6 +850,9 @@ int launch_bwd(BwdArgs a, hipStream_t st) {
   const Cut cut = bwd_cut(a.classes, Pack<T>::N == 4 ? VITTA_SCORES_F32 : VITTA_SCORES_BF16);
   a.segments = cut.segments, a.per_segment = cut.per_segment;
   const int64_t units = a.rows * cut.segments;
+  // A gradient of 512 MiB and more is streamed past the 256 MiB cache (2048 x 131072 bfloat16 188 -> 180 us); a smaller one stays in it, for the
+  // store itself and for who reads it next (1024 x 131072 87 -> 91 us, 1024 x 50021 floats 58 -> 75 if it were streamed).
+  a.stream_out = a.rows * a.classes * (int64_t)sizeof(T) >= (512ll << 20);
   if (a.classes <= kWaveRow) VITTA_LAUNCH((scores_grad_kernel<T, 64, DISTILL, ENT>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
   else VITTA_LAUNCH((scores_grad_kernel<T, 256, DISTILL, ENT>), dim3((unsigned)units), dim3(256), 0, st, a);
   return VITTA_OK;
