@@ -891,8 +891,9 @@ int vitta_frames_cv2_resize(const uint8_t* d_frames, int32_t n_frames, int32_t i
  *           where the student gives these nothing)
  *   d_q [rows][list], d_stats [rows][4]  for the backward.    list <= VITTA_SCORES_MAX_LIST
  * vitta_top_distill_bwd: d_dx [rows][classes] from d_g, a float per row at stride g_stride.
- * Workspace: vitta_scores_workspace_bytes(rows, classes, dtype, top) (top = 0 for the distillation), 256-byte aligned, may be 0;
- * one call's own until its launches have run.
+ * Workspace: vitta_scores_workspace_bytes(rows, classes, dtype, top) (top = 0 for the distillation), 16-byte aligned; one call's own until
+ * its launches have run.  0 unless few long rows are cut into segments; these are joined by a second launch, or, with d_tickets (rows
+ * uint32, zero when first used, left zero, not shared by launches that may run concurrently: one per stream), by the first one.
  * -------------------------------------------------------------------------- */
 #define VITTA_SCORES_F32 0
 #define VITTA_SCORES_BF16 1
@@ -903,7 +904,7 @@ size_t vitta_scores_workspace_bytes(int64_t rows, int32_t classes, int32_t dtype
 int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
                              const int64_t* d_labels, int64_t ignore_index, int32_t top, float* d_logprob, float* d_entropy,
                              float* d_lse, float* d_top_logprob, int64_t* d_top_index, float* d_stats, void* d_workspace,
-                             size_t workspace_bytes, void* stream);
+                             size_t workspace_bytes, uint32_t* d_tickets, void* stream);
 int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
                              const int64_t* d_labels, int64_t ignore_index, int32_t top, const int64_t* d_top_index,
                              const float* d_stats, const float* d_glogprob, int64_t glogprob_stride, const float* d_gentropy,
@@ -911,7 +912,7 @@ int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32
                              void* stream);
 int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
                           const int64_t* d_index, const void* d_value, int32_t value_dtype, int32_t list, int32_t tail, float* d_loss,
-                          float* d_stats, float* d_q, void* d_workspace, size_t workspace_bytes, void* stream);
+                          float* d_stats, float* d_q, void* d_workspace, size_t workspace_bytes, uint32_t* d_tickets, void* stream);
 int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
                           const int64_t* d_index, int32_t list, const float* d_stats, const float* d_q, const float* d_g,
                           int64_t g_stride, void* d_dx, void* stream);

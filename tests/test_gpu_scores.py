@@ -507,6 +507,38 @@ def test_repeats_streams_and_graphs(rows, classes):
         torch.rand(1000, device=DEV).sum().item()
 
 
+@pytest.mark.parametrize("rows,classes,top", [(1, 131072, 20), (3, 50001, 64), (200, 20001, 0), (511, 17000, 3)])
+def test_segments_join_in_one_launch_or_two(rows, classes, top, monkeypatch):
+    """Equal bits whether the last segment joins a row or a second launch does, many times over, on streams side by side; and the tickets
+    are zero afterwards."""
+    from vitta_amd import _lib, ops
+    x = [_scores(rows, classes, torch.bfloat16, 70 + i)[0] for i in range(3)]
+    labels = torch.arange(rows, device=DEV)
+    index, value = _list(rows, classes, 9, 71, True)
+    index, value = index.to(DEV), value.to(DEV)
+    assert _lib.lib().vitta_scores_workspace_bytes(rows, classes, 1, top) > 0
+
+    def step(x):
+        o = ops.label_logprobs(x, labels, top=top, lse=True)
+        return [t for t in o if t is not None] + [ops.top_distill(x, index, value, tail=True)]
+
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        want = [step(a) for a in x]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for turn in range(20):
+        got = []
+        for a, s in zip(x, streams):
+            with torch.cuda.stream(s):
+                got.append(step(a))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            for u, v in zip(a, b):
+                assert torch.equal(u, v)
+    assert len(ops._score_tickets) >= 3 and all(int(t.abs().sum()) == 0 for t in ops._score_tickets.values())
+
+
 def test_refusals():
     from vitta_amd import _lib, ops
     dx, _ = _scores(4, 50, torch.float32, 60)

@@ -74,7 +74,7 @@ def test_operators_refuse_host_tensors():
 
 def _fwd(**kw):
     a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, t=1.0, labels=4096, ignore=-100, top=0, logprob=4096, entropy=None, lse=4096,
-             top_logprob=None, top_index=None, stats=None, ws=None, ws_bytes=1 << 40)
+             top_logprob=None, top_index=None, stats=None, ws=None, ws_bytes=1 << 40, tickets=None)
     a.update(kw)
     return _lib.lib().vitta_label_logprobs_fwd(*a.values(), None)
 
@@ -108,7 +108,7 @@ def test_readout_gradient_refusals(bad):
 
 def _distil(**kw):
     a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, t=1.0, index=4096, value=4096, value_dtype=0, list=3, tail=0, loss=4096,
-             stats=4096, q=4096, ws=None, ws_bytes=1 << 40)
+             stats=4096, q=4096, ws=None, ws_bytes=1 << 40, tickets=None)
     a.update(kw)
     return _lib.lib().vitta_top_distill_fwd(*a.values(), None)
 

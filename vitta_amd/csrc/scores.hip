@@ -257,8 +257,9 @@ struct FwdArgs {
   int32_t classes, segments, per_segment;
   float c, inv_t;
   float* stats;
-  float4* part;     // [rows][segments] (m, s, t) of a segment
-  uint64_t* keys;   // [rows][segments][top]
+  float4* part;       // [rows][segments] (m, s, t) of a segment
+  uint64_t* keys;     // [rows][segments][top]
+  uint32_t* tickets;  // [rows] segments that are done, 0 at rest; NULL: a launch of its own joins them
   // readout
   const int64_t* labels;
   int64_t ignore;
@@ -392,6 +393,43 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
   reinterpret_cast<float4*>(A.stats)[row] = some ? st : make_float4(m, 0.f, m, 0.f);
 }
 
+// ---- the segments of a row ----------------------------------------------------------------------------------------------------------------
+// Their sums and lists pass through memory past the XCDs' caches: stored and loaded at device scope.
+template <typename V> __device__ __forceinline__ void put(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V> __device__ __forceinline__ V get(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// NW waves merge the lists (64 keys at a time, four loads ahead), the first one the sums
+template <typename T, int MODE, bool TOP, int NW>
+__device__ void join_segments(const FwdArgs& A, int64_t row, uint64_t* lists, int lane, int wave) {
+  const T* x = static_cast<const T*>(A.x) + row * A.stride;
+  Best best{0, false};
+  if (TOP) {
+    const int all = A.segments * A.top;
+    const uint64_t* keys = A.keys + row * all;
+    for (int at = wave * 64; at < all; at += 4 * NW * 64) {
+      uint64_t key[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) key[i] = at + i * NW * 64 + lane < all ? get(keys + at + i * NW * 64 + lane) : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at + i * NW * 64 < all) best.take(key[i], min(all - at - i * NW * 64, 64), lane);
+    }
+    lists[wave * 64 + lane] = best.mine;
+    __syncthreads();
+  }
+  if (wave != 0) return;
+  if (TOP)
+    for (int w = 1; w < NW && w * 64 < A.segments * A.top; ++w) best.mine = merge64(best.mine, lists[w * 64 + 63 - lane], lane);
+  Sum v{kLowest, 0.f, 0.f};
+  if (lane < A.segments) {
+    const float* p = reinterpret_cast<const float*>(A.part + row * A.segments + lane);
+    v = Sum{get(p), get(p + 1), get(p + 2)};
+  }
+  v = wave_merge(v, A.c, lane);
+  if (MODE == kReadout) finish_readout<T>(A, row, x, v, best.mine, lane);
+  else finish_distill<T, MODE == kDistillTail>(A, row, x, v, lane);
+}
+
 // ---- forward ---------------------------------------------------------------------------------------------------------------------------
 // NW waves share a (segment of a) row; with NW == 1 the four waves of a workgroup take four rows.
 template <typename T, int NW, int MODE, bool ENT, bool TOP>
@@ -399,7 +437,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
   constexpr int N = Pack<T>::N, NT = NW * 64, G = NW == 1 ? 4 : 1;  // G groups in a workgroup
   extern __shared__ __attribute__((aligned(16))) uint32_t bits_all[];  // kDistillTail: one bit per class of the group's segment
   __shared__ uint64_t keys_all[TOP ? (NW == 1 ? G : NW) * kKeys : 1];  // the waves' candidates, later their lists
-  __shared__ int counts[NW];
+  __shared__ int counts[NW], last_all;
   __shared__ Sum red[NW];
   __shared__ float bounds[NW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = NW == 1 ? lane : threadIdx.x;
@@ -600,13 +638,33 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
     }
   }
   if (NW > 1) {
-    if (wave != 0) return;
-    v = lane < NW ? red[lane] : Sum{kLowest, 0.f, 0.f};
-    v = wave_merge(v, c, lane);
+    if (wave != 0 && !(TOP && A.segments > 1)) return;
+    if (wave == 0) {
+      v = lane < NW ? red[lane] : Sum{kLowest, 0.f, 0.f};
+      v = wave_merge(v, c, lane);
+    }
     if (A.segments > 1) {
-      const int64_t at = row * A.segments + seg;
-      if (lane == 0) A.part[at] = make_float4(v.m, v.s, v.t, 0.f);
-      if (TOP && lane < A.top) A.keys[at * A.top + lane] = best.mine;
+      int last = 0;
+      if (wave == 0) {
+        const int64_t at = row * A.segments + seg;
+        float* p = reinterpret_cast<float*>(A.part + at);
+        if (lane == 0) put(p, v.m), put(p + 1, v.s), put(p + 2, v.t);
+        if (TOP && lane < A.top) put(A.keys + at * A.top + lane, best.mine);
+        if (A.tickets) {  // who comes last joins the row: what it reads was in memory before the others took their tickets
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          if (lane == 0) {
+            last = __hip_atomic_fetch_add(A.tickets + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)A.segments - 1;
+            if (last) put(A.tickets + row, 0u);
+          }
+          last = __builtin_amdgcn_readfirstlane(last);
+        }
+        if (TOP && lane == 0) last_all = last;
+      }
+      if (TOP) {
+        __syncthreads();
+        last = last_all;
+      }
+      if (last) join_segments<T, MODE, TOP, TOP ? NW : 1>(A, row, keys_all, lane, wave);
       return;
     }
   }
@@ -614,33 +672,11 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
   else finish_distill<T, MODE == kDistillTail>(A, row, whole, v, lane);
 }
 
-// joins the segments of a row: four waves merge the lists, the first one the sums
+// a launch of its own for the joins
 template <typename T, int MODE, bool TOP>
 __global__ __launch_bounds__(256) void scores_join_kernel(FwdArgs A) {
   __shared__ uint64_t lists[4 * 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(A.x) + row * A.stride;
-  uint64_t mine = 0;
-  if (TOP) {
-    for (int s = wave; s < A.segments; s += 4) {
-      const uint64_t o = 63 - lane < A.top ? A.keys[(row * A.segments + s) * A.top + 63 - lane] : 0;
-      mine = merge64(mine, o, lane);
-    }
-    lists[threadIdx.x] = mine;
-    __syncthreads();
-  }
-  if (wave != 0) return;
-  if (TOP)
-    for (int w = 1; w < 4; ++w) mine = merge64(mine, lists[w * 64 + 63 - lane], lane);
-  Sum v{kLowest, 0.f, 0.f};
-  if (lane < A.segments) {
-    const float4 p = A.part[row * A.segments + lane];
-    v = Sum{p.x, p.y, p.z};
-  }
-  v = wave_merge(v, A.c, lane);
-  if (MODE == kReadout) finish_readout<T>(A, row, x, v, mine, lane);
-  else finish_distill<T, MODE == kDistillTail>(A, row, x, v, lane);
+  join_segments<T, MODE, TOP, 4>(A, blockIdx.x, lists, threadIdx.x & 63, threadIdx.x >> 6);
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------------------------
@@ -819,7 +855,7 @@ bool too_large(int64_t rows, int32_t classes, int32_t type) {
 }
 
 template <typename T, int MODE, bool ENT, bool TOP>
-int launch_fwd(FwdArgs a, void* ws, hipStream_t st) {
+int launch_fwd(FwdArgs a, void* ws, uint32_t* tickets, hipStream_t st) {
   const Cut cut = fwd_cut(a.rows, a.classes);
   a.segments = cut.segments, a.per_segment = cut.per_segment;
   const size_t bits = MODE == kDistillTail ? ((size_t)(cut.per_segment + 16 + 31) / 32 + 1) * 4 : 0;
@@ -830,19 +866,20 @@ int launch_fwd(FwdArgs a, void* ws, hipStream_t st) {
   if (cut.segments > 1) {
     a.part = static_cast<float4*>(ws);
     a.keys = reinterpret_cast<uint64_t*>(a.part + a.rows * cut.segments);
+    a.tickets = tickets;
   }
   constexpr int NW = waves_of(TOP);
   VITTA_LAUNCH((scores_kernel<T, NW, MODE, ENT, TOP>), dim3((unsigned)(a.rows * cut.segments)), dim3(NW * 64), bits, st, a);
-  if (cut.segments > 1) VITTA_LAUNCH((scores_join_kernel<T, MODE, TOP>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  if (cut.segments > 1 && !tickets) VITTA_LAUNCH((scores_join_kernel<T, MODE, TOP>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
   return VITTA_OK;
 }
 
 template <int MODE, bool ENT, bool TOP>
-int launch_fwd(int32_t type, const FwdArgs& a, void* ws, void* stream) {
+int launch_fwd(int32_t type, const FwdArgs& a, void* ws, uint32_t* tickets, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (type == VITTA_SCORES_F32) return launch_fwd<float, MODE, ENT, TOP>(a, ws, st);
-  if (type == VITTA_SCORES_BF16) return launch_fwd<__hip_bfloat16, MODE, ENT, TOP>(a, ws, st);
-  return launch_fwd<_Float16, MODE, ENT, TOP>(a, ws, st);
+  if (type == VITTA_SCORES_F32) return launch_fwd<float, MODE, ENT, TOP>(a, ws, tickets, st);
+  if (type == VITTA_SCORES_BF16) return launch_fwd<__hip_bfloat16, MODE, ENT, TOP>(a, ws, tickets, st);
+  return launch_fwd<_Float16, MODE, ENT, TOP>(a, ws, tickets, st);
 }
 
 template <typename T, bool DISTILL, bool ENT>
@@ -879,7 +916,7 @@ size_t vitta_scores_workspace_bytes(int64_t rows, int32_t classes, int32_t dtype
 int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
                              const int64_t* d_labels, int64_t ignore_index, int32_t top, float* d_logprob, float* d_entropy,
                              float* d_lse, float* d_top_logprob, int64_t* d_top_index, float* d_stats, void* d_workspace,
-                             size_t workspace_bytes, void* stream) {
+                             size_t workspace_bytes, uint32_t* d_tickets, void* stream) {
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (top < 0 || top > VITTA_SCORES_MAX_TOP || top > classes || (top > 0 && (!d_top_logprob || !d_top_index))) return VITTA_ERR_INVALID_ARG;
   if (!d_labels != !d_logprob || (!d_logprob && !d_entropy && !d_lse && top == 0)) return VITTA_ERR_INVALID_ARG;
@@ -891,8 +928,8 @@ int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32
   a.x = d_x, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.labels = d_labels, a.ignore = ignore_index, a.top = top, a.logprob = d_logprob, a.entropy = d_entropy, a.lse = d_lse;
   a.top_logprob = d_top_logprob, a.top_index = d_top_index;
-  if (d_entropy) return top ? launch_fwd<kReadout, true, true>(dtype, a, d_workspace, stream) : launch_fwd<kReadout, true, false>(dtype, a, d_workspace, stream);
-  return top ? launch_fwd<kReadout, false, true>(dtype, a, d_workspace, stream) : launch_fwd<kReadout, false, false>(dtype, a, d_workspace, stream);
+  if (d_entropy) return top ? launch_fwd<kReadout, true, true>(dtype, a, d_workspace, d_tickets, stream) : launch_fwd<kReadout, true, false>(dtype, a, d_workspace, d_tickets, stream);
+  return top ? launch_fwd<kReadout, false, true>(dtype, a, d_workspace, d_tickets, stream) : launch_fwd<kReadout, false, false>(dtype, a, d_workspace, d_tickets, stream);
 }
 
 int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
@@ -913,7 +950,7 @@ int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32
 
 int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
                           const int64_t* d_index, const void* d_value, int32_t value_dtype, int32_t list, int32_t tail, float* d_loss,
-                          float* d_stats, float* d_q, void* d_workspace, size_t workspace_bytes, void* stream) {
+                          float* d_stats, float* d_q, void* d_workspace, size_t workspace_bytes, uint32_t* d_tickets, void* stream) {
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || !d_value || !d_loss || bad_stats(d_stats) || !d_q || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
   if (value_dtype < VITTA_SCORES_F32 || value_dtype > VITTA_SCORES_F16) return VITTA_ERR_INVALID_ARG;
@@ -924,7 +961,7 @@ int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t 
   a.x = d_x, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.index = d_index, a.value = d_value, a.value_type = value_dtype, a.list = list;
   a.loss = d_loss, a.q = d_q;
-  return tail ? launch_fwd<kDistillTail, false, false>(dtype, a, d_workspace, stream) : launch_fwd<kDistill, false, false>(dtype, a, d_workspace, stream);
+  return tail ? launch_fwd<kDistillTail, false, false>(dtype, a, d_workspace, d_tickets, stream) : launch_fwd<kDistill, false, false>(dtype, a, d_workspace, d_tickets, stream);
 }
 
 int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,

@@ -211,9 +211,24 @@ def _score_workspace_bytes(rows, classes, dtype, top):
     return int(lib().vitta_scores_workspace_bytes(rows, classes, dtype, top))
 
 
+_score_tickets = {}  # (device index, stream): zeros, left zero by the launches that use them
+
+
 def _score_workspace(m, rows, classes, top):
+    """(workspace or None, its bytes, tickets' address or None) of a call.  Segments of long rows meet on tickets that belong to the current
+    stream; a captured call has none (two graphs of one stream may be replayed side by side) and joins them in a second launch."""
     n = _score_workspace_bytes(rows, classes, _SCORE_TYPES[m.dtype], top)
-    return (m.new_empty(n, dtype=torch.uint8) if n else None), n
+    if not n:
+        return None, 0, None
+    ws = m.new_empty(n, dtype=torch.uint8)
+    index = m.device.index
+    if rows > 512 or index != torch._C._cuda_getDevice() or torch.cuda.is_current_stream_capturing():
+        return ws, n, None
+    key = (index, torch._C._cuda_getCurrentRawStream(index))
+    tickets = _score_tickets.get(key)
+    if tickets is None:
+        tickets = _score_tickets[key] = torch.zeros(512, dtype=torch.int32, device=m.device)
+    return ws, n, tickets.data_ptr()
 
 
 def _row_gradient(g, rows):
@@ -236,9 +251,9 @@ def _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_inde
     top_logprob = m.new_empty((*lead, top), dtype=f32) if top else None
     top_index = m.new_empty((*lead, top), dtype=torch.int64) if top else None
     if rows:
-        ws, n = _score_workspace(m, rows, classes, top)
+        ws, n, tickets = _score_workspace(m, rows, classes, top)
         _call("vitta_label_logprobs_fwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _ptr(labels),
-              ignore_index, top, _ptr(logprob), _ptr(ent), _ptr(lse), _ptr(top_logprob), _ptr(top_index), _ptr(stats), _ptr(ws), n)
+              ignore_index, top, _ptr(logprob), _ptr(ent), _ptr(lse), _ptr(top_logprob), _ptr(top_index), _ptr(stats), _ptr(ws), n, tickets)
     return logprob, ent, lse, top_logprob, top_index
 
 
@@ -306,9 +321,9 @@ def _top_distill(m, lead, index, value, temperature, tail):
     loss = m.new_empty(lead, dtype=torch.float32)
     side = m.new_empty(rows * (4 + k), dtype=torch.float32)  # the row statistics (rows, 4), then the teacher's probabilities (rows, k)
     if rows:
-        ws, n = _score_workspace(m, rows, classes, 0)
+        ws, n, tickets = _score_workspace(m, rows, classes, 0)
         _call("vitta_top_distill_fwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, index.data_ptr(),
-              value.data_ptr(), _SCORE_TYPES[value.dtype], k, tail, loss.data_ptr(), side.data_ptr(), side.data_ptr() + 16 * rows, _ptr(ws), n)
+              value.data_ptr(), _SCORE_TYPES[value.dtype], k, tail, loss.data_ptr(), side.data_ptr(), side.data_ptr() + 16 * rows, _ptr(ws), n, tickets)
     return loss, side
 
 
