@@ -165,20 +165,22 @@ class LabelLogprobs(NamedTuple):
 
 # These calls are short (a batch of class scores is a few microseconds of GPU time), so their host side is kept lean: plain integers to
 # ctypes, the raw stream, a device switch only where the tensors are not on the current device.
-def _call(name, device, *args):
-    """check(name(*args, stream)) on the tensors' device and its current stream."""
-    fn = getattr(lib(), name)
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_entry_points = {}
+
+
+def _call(name, index, *args):
+    """check(name(*args, stream)) on device `index` and its current stream."""
+    fn = _entry_points.get(name)
+    if fn is None:
+        fn = _entry_points[name] = getattr(lib(), name)
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):  # (the library launches on the current device)
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    check(status, name)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+        with torch.cuda.device(index):  # (the library launches on the current device)
+            status = fn(*args, _raw_stream(index))
+    if status or _lib.CALL_COUNTS is not None:
+        check(status, name)
 
 
 def _score_rows(x, name, temperature):
@@ -214,27 +216,25 @@ def _score_workspace_bytes(rows, classes, dtype, top):
 _score_tickets = {}  # (device index, stream): zeros, left zero by the launches that use them
 
 
-def _score_workspace(m, rows, classes, top):
+def _score_workspace(m, rows, classes, dtype, top):
     """(workspace or None, its bytes, tickets' address or None) of a call.  Segments of long rows meet on tickets that belong to the current
     stream; a captured call has none (two graphs of one stream may be replayed side by side) and joins them in a second launch."""
-    n = _score_workspace_bytes(rows, classes, _SCORE_TYPES[m.dtype], top)
+    n = _score_workspace_bytes(rows, classes, dtype, top)
     if not n:
         return None, 0, None
     ws = m.new_empty(n, dtype=torch.uint8)
-    index = m.device.index
-    if rows > 512 or index != torch._C._cuda_getDevice() or torch.cuda.is_current_stream_capturing():
+    index = m.get_device()
+    if rows > 512 or index != _current_device() or torch.cuda.is_current_stream_capturing():
         return ws, n, None
-    key = (index, torch._C._cuda_getCurrentRawStream(index))
+    key = (index, _raw_stream(index))
     tickets = _score_tickets.get(key)
     if tickets is None:
         tickets = _score_tickets[key] = torch.zeros(512, dtype=torch.int32, device=m.device)
     return ws, n, tickets.data_ptr()
 
 
-def _row_gradient(g, rows):
-    """(tensor or None, stride) of an upstream gradient per row; one value for every row (what mean() and sum() send) is not spread out."""
-    if g is None:
-        return None, 0
+def _row_gradient(g):
+    """(tensor, stride) of an upstream gradient per row; one value for every row (what mean() and sum() send) is not spread out."""
     if g.is_contiguous():
         return g, 1
     if all(s == 0 or n == 1 for s, n in zip(g.stride(), g.shape)):
@@ -245,15 +245,27 @@ def _row_gradient(g, rows):
 def _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_index, stats):
     rows, classes = m.shape
     f32 = torch.float32
-    logprob = m.new_empty(lead, dtype=f32) if labels is not None else None
-    ent = m.new_empty(lead, dtype=f32) if entropy else None
-    lse = m.new_empty(lead, dtype=f32) if lse else None
-    top_logprob = m.new_empty((*lead, top), dtype=f32) if top else None
-    top_index = m.new_empty((*lead, top), dtype=torch.int64) if top else None
+    a = b = c = d = e = y = None
+    logprob = ent = top_logprob = top_index = None
+    if labels is not None:
+        logprob = m.new_empty(lead, dtype=f32)
+        a, y = logprob.data_ptr(), labels.data_ptr()
+    if entropy:
+        ent = m.new_empty(lead, dtype=f32)
+        b = ent.data_ptr()
+    if lse:
+        lse = m.new_empty(lead, dtype=f32)
+        c = lse.data_ptr()
+    else:
+        lse = None
+    if top:
+        top_logprob, top_index = m.new_empty((*lead, top), dtype=f32), m.new_empty((*lead, top), dtype=torch.int64)
+        d, e = top_logprob.data_ptr(), top_index.data_ptr()
     if rows:
-        ws, n, tickets = _score_workspace(m, rows, classes, top)
-        _call("vitta_label_logprobs_fwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _ptr(labels),
-              ignore_index, top, _ptr(logprob), _ptr(ent), _ptr(lse), _ptr(top_logprob), _ptr(top_index), _ptr(stats), _ptr(ws), n, tickets)
+        dtype = _SCORE_TYPES[m.dtype]
+        ws, n, tickets = _score_workspace(m, rows, classes, dtype, top)
+        _call("vitta_label_logprobs_fwd", m.get_device(), m.data_ptr(), dtype, rows, classes, m.stride(0), temperature, y, ignore_index, top,
+              a, b, c, d, e, None if stats is None else stats.data_ptr(), None if ws is None else ws.data_ptr(), n, tickets)
     return logprob, ent, lse, top_logprob, top_index
 
 
@@ -278,12 +290,24 @@ def _label_logprobs_grad(ctx, g_logprob, g_entropy, g_lse, g_top, _):
     m, labels, top_index, stats = ctx.saved_tensors
     top, temperature, ignore_index = ctx.how
     rows, classes = m.shape
-    dx = m.new_empty(m.shape)
+    dx = m.new_empty((rows, classes))
     if rows:
-        (a, sa), (b, sb), (c, sc) = _row_gradient(g_logprob, rows), _row_gradient(g_entropy, rows), _row_gradient(g_lse, rows)
-        g_top = g_top.contiguous() if g_top is not None else None
-        _call("vitta_label_logprobs_bwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, _ptr(labels),
-              ignore_index, top, _ptr(top_index), stats.data_ptr(), _ptr(a), sa, _ptr(b), sb, _ptr(c), sc, _ptr(g_top), dx.data_ptr())
+        a = b = c = d = e = y = None
+        sa = sb = sc = 0
+        if g_logprob is not None:
+            g_logprob, sa = _row_gradient(g_logprob)
+            a, y = g_logprob.data_ptr(), labels.data_ptr()
+        if g_entropy is not None:
+            g_entropy, sb = _row_gradient(g_entropy)
+            b = g_entropy.data_ptr()
+        if g_lse is not None:
+            g_lse, sc = _row_gradient(g_lse)
+            c = g_lse.data_ptr()
+        if g_top is not None:
+            g_top = g_top.contiguous()
+            d, e = g_top.data_ptr(), top_index.data_ptr()
+        _call("vitta_label_logprobs_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, y,
+              ignore_index, top, e, stats.data_ptr(), a, sa, b, sb, c, sc, d, dx.data_ptr())
     return dx, None, None, None, None, None, None, None
 
 
@@ -316,14 +340,18 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
 
 
 def _top_distill(m, lead, index, value, temperature, tail):
+    """(loss, the row statistics (rows, 4) and the teacher's probabilities (rows, k) in one buffer)"""
     rows, classes = m.shape
     k = index.shape[-1]
     loss = m.new_empty(lead, dtype=torch.float32)
-    side = m.new_empty(rows * (4 + k), dtype=torch.float32)  # the row statistics (rows, 4), then the teacher's probabilities (rows, k)
+    side = m.new_empty(rows * (4 + k), dtype=torch.float32)
     if rows:
-        ws, n, tickets = _score_workspace(m, rows, classes, 0)
-        _call("vitta_top_distill_fwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, index.data_ptr(),
-              value.data_ptr(), _SCORE_TYPES[value.dtype], k, tail, loss.data_ptr(), side.data_ptr(), side.data_ptr() + 16 * rows, _ptr(ws), n, tickets)
+        dtype = _SCORE_TYPES[m.dtype]
+        ws, n, tickets = _score_workspace(m, rows, classes, dtype, 0)
+        stats = side.data_ptr()
+        _call("vitta_top_distill_fwd", m.get_device(), m.data_ptr(), dtype, rows, classes, m.stride(0), temperature, index.data_ptr(),
+              value.data_ptr(), _SCORE_TYPES[value.dtype], k, tail, loss.data_ptr(), stats, stats + 16 * rows,
+              None if ws is None else ws.data_ptr(), n, tickets)
     return loss, side
 
 
@@ -343,11 +371,12 @@ class _TopDistill(torch.autograd.Function):
 def _top_distill_grad(ctx, g):
     m, index, side = ctx.saved_tensors
     rows, classes = m.shape
-    dx = m.new_empty(m.shape)
+    dx = m.new_empty((rows, classes))
     if rows:
-        g, sg = _row_gradient(g, rows)
-        _call("vitta_top_distill_bwd", m.device, m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), ctx.temperature,
-              index.data_ptr(), index.shape[-1], side.data_ptr(), side.data_ptr() + 16 * rows, g.data_ptr(), sg, dx.data_ptr())
+        g, sg = _row_gradient(g)
+        stats = side.data_ptr()
+        _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), ctx.temperature,
+              index.data_ptr(), index.shape[-1], stats, stats + 16 * rows, g.data_ptr(), sg, dx.data_ptr())
     return dx, None, None, None, None, None
 
 
