@@ -507,7 +507,7 @@ def test_repeats_streams_and_graphs(rows, classes):
         torch.rand(1000, device=DEV).sum().item()
 
 
-@pytest.mark.parametrize("rows,classes,top", [(1, 131072, 20), (3, 50001, 64), (200, 20001, 0), (511, 17000, 3)])
+@pytest.mark.parametrize("rows,classes,top", [(1, 131072, 20), (3, 50001, 64), (200, 40001, 0), (511, 17000, 3)])
 def test_segments_join_in_one_launch_or_two(rows, classes, top, monkeypatch):
     """Equal bits whether the last segment joins a row or a second launch does, many times over, on streams side by side; and the tickets
     are zero afterwards."""

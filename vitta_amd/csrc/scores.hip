@@ -7,14 +7,16 @@
 // m starts at the lowest finite float: a row of minus infinities keeps s = 0 and is answered as a row without a distribution.
 // Sums, maxima and statistics are 32 bits wide; a gradient is rounded once, to the scores' type.
 //
-// Forward: one pass.  A lane holds four 16-byte loads while the next four are on their way, takes their maximum, moves its running sums to
-// it and adds; the lanes' (m, s, t) are joined at the end.  A short row (<= kWaveRow classes) belongs to one wave, a longer one to a
-// workgroup of eight, and few long rows are cut into segments whose results a second launch joins.
-// Best alternatives in the same pass: a lower bound of the k-th best (from the lanes' maxima of the first loads) lets all but a few scores
-// pass by; the few go to a buffer of their wave in LDS, and every 64 of them are sorted across the lanes and merged into the wave's
-// list of 64.  Equal scores order by class, so the answer does not depend on which wave saw what.
-// Gradient: elementwise from the row statistics, e_j (A + B a_j); the few classes that a label or a list adds to are written again at the end
-// by the workgroup that wrote them.
+// Forward: one pass, bound by memory (4096 x 131072 bfloat16: 170 us = 6.3 TB/s with label and entropy, 200 us with 64 alternatives, where the
+// candidates' instructions add up; 2048 x 32003 float16 with 5: 36 us).  A lane holds four 16-byte loads while the next four are on
+// their way, takes their maximum, moves its running sums to it and adds; the lanes' (m, s, t) are joined at the end.  A short row belongs to
+// one wave, a longer one to a workgroup (wave_rows), and few long rows are cut into segments (fwd_cut) that the last one of a row joins.
+// Best alternatives in the same pass: a lower bound of the k-th best (from the lanes' maxima of the first loads, raised later) lets all but a
+// few scores pass by; these few wait with their classes in LDS, and at the end 64 at a time are sorted across the lanes of a wave and merged
+// into its list of 64.  Equal scores order by class, so the answer does not depend on which wave saw what.  (Sorting as they come,
+// or keeping only their classes and reading the scores again, took 330 and 297 us of the first case.)
+// Gradient: elementwise from the row statistics, e_j (A + B a_j), bound by memory (4096 x 131072 bfloat16: 356 us = 6.0 TB/s); the few classes
+// that a label or a list adds to are written again at the end by the workgroup that wrote them.
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -31,7 +33,9 @@ constexpr int kU = 4;              // 16-byte loads of a lane that are consumed 
 // Waves of a workgroup that share a long row: eight, four where it collects alternatives (2048 x 32003 float16: 27.0 us with eight and 29.5 with four
 // without alternatives, 40.3 and 36.5 with five of them; 4096 x 131072 bfloat16 with 64 of them 223 and 203).
 constexpr int waves_of(bool top) { return top ? 4 : 8; }
-constexpr int kWaveRow = 4096;     // classes up to which a row belongs to one wave
+constexpr int kWaveRow = 4096;     // classes up to which a row may belong to one wave, in the forward
+constexpr int kWaveGrad = 2048;    // and does, in the gradient
+constexpr int kWorkgroups = 512;   // workgroups that few long rows are cut into (1024: 400 x 131072 27 -> 25 us, 64 x 131072 with alternatives 15 -> 17)
 constexpr int kKeys = 256;         // candidates that a wave keeps: 2 KiB of LDS
 constexpr int kMaxSegments = 64;
 constexpr int kTailSegment = 1 << 18;  // classes whose membership bits fit 32 KiB
@@ -701,7 +705,7 @@ struct BwdArgs {
 };
 
 // dx_j = e_j (a0 + a1 a_j), with a0 = at0 for the classes of the group's list, to which it adds `add`.
-// A workgroup takes what its threads hold in kU loads each (32 KiB with what it writes), a wave a row of up to kWaveRow classes.
+// A workgroup takes what its threads hold in kU loads each (32 KiB with what it writes), a wave a row of up to kWaveGrad classes.
 template <typename T, int NT, bool DISTILL, bool ENT>
 __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
   constexpr int N = Pack<T>::N, G = 256 / NT, L = DISTILL ? VITTA_SCORES_MAX_LIST : VITTA_SCORES_MAX_TOP + 1;
@@ -832,34 +836,39 @@ Cut cut_into(int32_t classes, int64_t segments) {
   per = (per + 511) / 512 * 512;  // (whole 16-byte vectors: a segment starts as the row is aligned)
   return Cut{(int32_t)((classes + per - 1) / per), (int32_t)per};
 }
-// Segments of a row in the forward: enough workgroups for the chip, none of fewer than 8192 classes.
-Cut fwd_cut(int64_t rows, int32_t classes) {
-  if (classes <= kWaveRow) return Cut{1, classes};
-  int64_t s = (512 + rows - 1) / rows;
-  s = s < classes / 8192 ? s : classes / 8192;
+// Whether a row of the forward belongs to one wave.  Up to 1024 classes it always does, up to kWaveRow where there are rows for every wave or no
+// alternatives to sort, which four waves do in a quarter of the time (512 x 4000 bfloat16 with 20 alternatives: 10.6 us by waves, 6.7 by
+// workgroups; 8192 x 4000: 27.0 and 30.1; without alternatives 512 x 4000: 4.9 and 4.7, 8192 x 4000: 16.7 and 24.3).
+bool wave_rows(int64_t rows, int32_t classes, bool top) { return classes <= 1024 || (classes <= kWaveRow && (!top || rows >= 2048)); }
+// Segments of a row in the forward: enough workgroups for the chip, none with less than one step of its threads.
+Cut fwd_cut(int64_t rows, int32_t classes, int32_t type, bool top) {
+  if (wave_rows(rows, classes, top)) return Cut{1, classes};
+  int64_t s = (kWorkgroups + rows - 1) / rows;
+  const int32_t floor = top || type == VITTA_SCORES_F32 ? 8192 : 16384;
+  s = s < classes / floor ? s : classes / floor;
   s = s > kMaxSegments ? kMaxSegments : s;
   const int64_t least = ((int64_t)classes + kTailSegment - 1) / kTailSegment;  // (membership bits)
   s = s < least ? least : s;
   return s <= 1 ? Cut{1, classes} : cut_into(classes, s);
 }
-// A workgroup of the gradient takes one load of its 256 threads: 16 KiB of a row (2 x 32 KiB: 4096 x 131072 bfloat16 360 -> 381 us).
+// A row of the gradient of up to 2048 classes belongs to one wave (512 x 4000 bfloat16: 6.0 us by waves, 4.6 by workgroups; 512 x 2000: 4.9 and
+// 4.8), a workgroup takes one load of its 256 threads, 16 KiB of a row (2 x 32 KiB: 4096 x 131072 bfloat16 360 -> 381 us).
 Cut bwd_cut(int32_t classes, int32_t type) {
   const int32_t per = 256 * kU * (type == VITTA_SCORES_F32 ? 4 : 8);
-  return classes <= kWaveRow || classes <= per ? Cut{1, classes} : Cut{(int32_t)(((int64_t)classes + per - 1) / per), per};
+  return classes <= kWaveGrad || classes <= per ? Cut{1, classes} : Cut{(int32_t)(((int64_t)classes + per - 1) / per), per};
 }
-
 // sizes a launch does not take: more workgroups than a grid has, rows that no 64 segments of kTailSegment hold
-bool too_large(int64_t rows, int32_t classes, int32_t type) {
+bool too_large(int64_t rows, int32_t classes, int32_t type, bool top) {
   if (classes > kMaxSegments * kTailSegment || rows > 0x7fffffff) return true;
-  return rows * (int64_t)fwd_cut(rows, classes).segments > 0x7fffffff || rows * (int64_t)bwd_cut(classes, type).segments > 0x7fffffff;
+  return rows * (int64_t)fwd_cut(rows, classes, type, top).segments > 0x7fffffff || rows * (int64_t)bwd_cut(classes, type).segments > 0x7fffffff;
 }
 
 template <typename T, int MODE, bool ENT, bool TOP>
 int launch_fwd(FwdArgs a, void* ws, uint32_t* tickets, hipStream_t st) {
-  const Cut cut = fwd_cut(a.rows, a.classes);
+  const Cut cut = fwd_cut(a.rows, a.classes, Pack<T>::N == 4 ? VITTA_SCORES_F32 : VITTA_SCORES_BF16, TOP);
   a.segments = cut.segments, a.per_segment = cut.per_segment;
   const size_t bits = MODE == kDistillTail ? ((size_t)(cut.per_segment + 16 + 31) / 32 + 1) * 4 : 0;
-  if (a.classes <= kWaveRow) {
+  if (wave_rows(a.rows, a.classes, TOP)) {
     VITTA_LAUNCH((scores_kernel<T, 1, MODE, ENT, TOP>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 4 * bits, st, a);
     return VITTA_OK;
   }
@@ -890,7 +899,7 @@ int launch_bwd(BwdArgs a, hipStream_t st) {
   // A gradient of 512 MiB and more is streamed past the 256 MiB cache (2048 x 131072 bfloat16 188 -> 180 us); a smaller one stays in it, for the
   // store itself and for who reads it next (1024 x 131072 87 -> 91 us, 1024 x 50021 floats 58 -> 75 if it were streamed).
   a.stream_out = a.rows * a.classes * (int64_t)sizeof(T) >= (512ll << 20);
-  if (a.classes <= kWaveRow) VITTA_LAUNCH((scores_grad_kernel<T, 64, DISTILL, ENT>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
+  if (a.classes <= kWaveGrad) VITTA_LAUNCH((scores_grad_kernel<T, 64, DISTILL, ENT>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
   else VITTA_LAUNCH((scores_grad_kernel<T, 256, DISTILL, ENT>), dim3((unsigned)units), dim3(256), 0, st, a);
   return VITTA_OK;
 }
@@ -908,8 +917,8 @@ int launch_bwd(int32_t type, const BwdArgs& a, void* stream) {
 extern "C" {
 
 size_t vitta_scores_workspace_bytes(int64_t rows, int32_t classes, int32_t dtype, int32_t top) {
-  if (rows <= 0 || classes <= 0 || top < 0 || top > VITTA_SCORES_MAX_TOP || too_large(rows, classes, dtype)) return 0;
-  const int64_t s = fwd_cut(rows, classes).segments;
+  if (rows <= 0 || classes <= 0 || top < 0 || top > VITTA_SCORES_MAX_TOP || too_large(rows, classes, dtype, top > 0)) return 0;
+  const int64_t s = fwd_cut(rows, classes, dtype, top > 0).segments;
   return s == 1 ? 0 : (size_t)rows * s * (16 + 8 * (size_t)top);
 }
 
@@ -921,7 +930,7 @@ int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32
   if (top < 0 || top > VITTA_SCORES_MAX_TOP || top > classes || (top > 0 && (!d_top_logprob || !d_top_index))) return VITTA_ERR_INVALID_ARG;
   if (!d_labels != !d_logprob || (!d_logprob && !d_entropy && !d_lse && top == 0)) return VITTA_ERR_INVALID_ARG;
   if (d_stats && bad_stats(d_stats)) return VITTA_ERR_INVALID_ARG;
-  if (too_large(rows, classes, dtype)) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes, dtype, top > 0)) return VITTA_ERR_UNSUPPORTED;
   const size_t need = vitta_scores_workspace_bytes(rows, classes, dtype, top);
   if (workspace_bytes < need || (need && bad_stats(d_workspace))) return VITTA_ERR_WORKSPACE;
   FwdArgs a{};
@@ -939,7 +948,7 @@ int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32
                              void* stream) {
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature) || bad_stats(d_stats) || bad_out(d_dx, dtype)) return VITTA_ERR_INVALID_ARG;
   if ((d_glogprob && !d_labels) || (d_gtop && (!d_top_index || top <= 0 || top > VITTA_SCORES_MAX_TOP))) return VITTA_ERR_INVALID_ARG;
-  if (too_large(rows, classes, dtype)) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes, dtype, false)) return VITTA_ERR_UNSUPPORTED;
   BwdArgs a{};
   a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.labels = d_labels, a.ignore = ignore_index, a.top = top, a.top_index = d_top_index;
@@ -954,7 +963,7 @@ int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t 
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || !d_value || !d_loss || bad_stats(d_stats) || !d_q || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
   if (value_dtype < VITTA_SCORES_F32 || value_dtype > VITTA_SCORES_F16) return VITTA_ERR_INVALID_ARG;
-  if (too_large(rows, classes, dtype)) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes, dtype, false)) return VITTA_ERR_UNSUPPORTED;
   const size_t need = vitta_scores_workspace_bytes(rows, classes, dtype, 0);
   if (workspace_bytes < need || (need && bad_stats(d_workspace))) return VITTA_ERR_WORKSPACE;
   FwdArgs a{};
@@ -969,7 +978,7 @@ int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t 
                           int64_t g_stride, void* d_dx, void* stream) {
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || bad_stats(d_stats) || !d_q || !d_g || bad_out(d_dx, dtype) || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
-  if (too_large(rows, classes, dtype)) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes, dtype, false)) return VITTA_ERR_UNSUPPORTED;
   BwdArgs a{};
   a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.index = d_index, a.list = list, a.q = d_q, a.g = d_g, a.s_g = g_stride;
