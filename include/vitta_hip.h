@@ -873,20 +873,20 @@ int vitta_frames_cv2_resize(const uint8_t* d_frames, int32_t n_frames, int32_t i
 /* --------------------------------------------------------------------------
  * Rows of class scores (logits): what they say of a label, how sure they are, and a loss against another model's answer.
  *   d_x     [rows][row_stride] scores, classes of them used per row (row_stride in elements, any >= 0); dtype one of the
- *           VITTA_SCORES_* below, element aligned;  z = x / temperature,  p = softmax(z)
+ *           VITTA_SCORES_* below, element aligned; at most 2^24 classes and 2^31 - 1 rows;  z = x / temperature,  p = softmax(z)
  * vitta_label_logprobs_fwd, any of the outputs may be NULL:
  *   d_logprob [rows]      z_y - lse of label y = d_labels[row]; 0 where y == ignore_index, NaN where y is no class (nothing is read)
  *   d_entropy [rows]      -sum p log p        d_lse [rows]  log sum exp z
  *   d_top_logprob, d_top_index [rows][top]    the `top` highest scores in falling order, ties to the lowest class; index -1 (and log
  *                         probability -inf) where fewer classes have a score above -inf.  top <= VITTA_SCORES_MAX_TOP, <= classes
- *   d_stats [rows][4]     row statistics for the backward (16-byte aligned)
+ *   d_stats [rows][4]     row statistics for the backward (16-byte aligned); for one with d_gentropy the call needs d_entropy
  *   A row of -inf only: log probabilities -inf, entropy 0, gradient 0.  A row with a NaN or +inf: NaN everywhere, indices -1.
  * vitta_label_logprobs_bwd: d_dx [rows][classes] (dtype, dense) from the upstream gradients, each NULL or a float per row at the given
  *   element stride (0: one value for every row); d_gtop [rows][top] dense.  A row whose upstream gradients are all 0 gets zeros.
  * vitta_top_distill_fwd: d_loss[row] = KL(teacher's list || student)
  *   d_index, d_value [rows][list]  the teacher's classes and scores; an index that is no class (-1) is padding; a row of padding only
  *           has loss 0 and gradient 0.  A class listed twice counts with the sum of its probabilities.
- *   tail == 0: q = softmax(d_value / temperature) over the list
+ *   tail == 0: q = softmax(d_value / temperature) over the list (NaN for a list of -inf only)
  *   tail != 0: d_value are log probabilities; what they leave of 1 belongs to the classes outside the list as one class (left out
  *           where the student gives these nothing)
  *   d_q [rows][list], d_stats [rows][4]  for the backward.    list <= VITTA_SCORES_MAX_LIST

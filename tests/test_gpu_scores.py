@@ -456,6 +456,26 @@ def test_far_offsets():
         _check_grad(grad[r:r + 1], want, bound, torch.bfloat16)
 
 
+def test_more_rows_than_one_launch_takes():
+    """Millions of rows (of stride 0, so that they need no memory): launches of 2^31 threads at most follow one another."""
+    from vitta_amd import ops
+    for rows, classes, top in ((4_200_000, 5000, 0), (8_400_005, 4500, 2)):
+        x = _scores(1, classes, torch.bfloat16, classes)[1]
+        got = ops.label_logprobs(x.to(DEV).expand(rows, classes), top=top)
+        assert torch.equal(got.entropy, got.entropy[:1].expand(rows))
+        if top:
+            assert torch.equal(got.top_index, got.top_index[:1].expand(rows, top))
+        _check_readout(ops.LabelLogprobs(*[None if t is None else t[-1:] for t in got]), x, None, top, 1.0)
+    rows, classes = 8_400_005, 2049
+    x = _scores(1, classes, torch.bfloat16, 3)[1]
+    wide = x.to(DEV).expand(rows, classes).requires_grad_()
+    (grad,) = torch.autograd.grad(ops.label_logprobs(wide).entropy.sum(), wide)
+    want, bound = O.readout_grad(x, None, 0, 1.0, None, torch.ones(1))
+    for r in (0, 8_388_604, 8_388_608, rows - 1):
+        _check_grad(grad[r:r + 1], want, bound, torch.bfloat16)
+    assert torch.equal(grad[-1], grad[0]) and bool((grad[::1000] == grad[0]).all())
+
+
 @pytest.mark.parametrize("rows,classes", [(1, 131072), (40, 101), (300, 9001)])
 def test_repeats_streams_and_graphs(rows, classes):
     """Equal bits on a second call, on another stream, and on every replay of a captured graph with other work in between."""

@@ -91,6 +91,7 @@ def test_readout_refusals(bad):
 
 def test_sizes_beyond_a_launch_are_refused():
     assert _fwd(rows=1 << 40) == -4
+    assert _fwd(classes=(1 << 24) + 1, stride=1 << 25) == -4
 
 
 def _bwd(**kw):

@@ -257,7 +257,7 @@ struct Best {
 // ---- arguments ---------------------------------------------------------------------------------------------------------------------
 struct FwdArgs {
   const void* x;
-  int64_t rows, stride;
+  int64_t rows, stride, row0;  // row0: the launch's first row
   int32_t classes, segments, per_segment;
   float c, inv_t;
   float* stats;
@@ -448,13 +448,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
   int64_t row;
   int seg = 0;
   if (NW == 1) {
-    row = (int64_t)blockIdx.x * G + wave;
+    row = A.row0 + (int64_t)blockIdx.x * G + wave;
     if (row >= A.rows) return;  // (no workgroup barrier in this form)
   } else if (A.segments == 1) {
-    row = blockIdx.x;
+    row = A.row0 + blockIdx.x;
   } else {
-    row = blockIdx.x / A.segments;
-    seg = blockIdx.x - (int)row * A.segments;
+    const uint32_t at = blockIdx.x / (uint32_t)A.segments;
+    row = A.row0 + at;
+    seg = (int)(blockIdx.x - at * (uint32_t)A.segments);
   }
   const T* whole = static_cast<const T*>(A.x) + row * A.stride;
   const int j0 = seg * A.per_segment, n = min(A.per_segment, A.classes - j0);
@@ -661,6 +662,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
             if (last) put(A.tickets + row, 0u);
           }
           last = __builtin_amdgcn_readfirstlane(last);
+          asm volatile("" ::: "memory");
         }
         if (TOP && lane == 0) last_all = last;
       }
@@ -680,14 +682,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
 template <typename T, int MODE, bool TOP>
 __global__ __launch_bounds__(256) void scores_join_kernel(FwdArgs A) {
   __shared__ uint64_t lists[4 * 64];
-  join_segments<T, MODE, TOP, 4>(A, blockIdx.x, lists, threadIdx.x & 63, threadIdx.x >> 6);
+  join_segments<T, MODE, TOP, 4>(A, A.row0 + blockIdx.x, lists, threadIdx.x & 63, threadIdx.x >> 6);
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------------------------
 struct BwdArgs {
   const void* x;
   void* dx;
-  int64_t rows, stride;
+  int64_t rows, stride, row0;
   int32_t classes, segments, per_segment;
   float c, inv_t;
   const float* stats;
@@ -715,10 +717,10 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
   const int group = threadIdx.x / NT, tid = threadIdx.x - group * NT, lane = threadIdx.x & 63;
   int32_t* at = at_all + group * L;
   float* add = add_all + group * L;
-  const int64_t unit = (int64_t)blockIdx.x * G + group;
-  const int64_t row = A.segments == 1 ? unit : unit / A.segments;
+  const uint32_t unit = G > 1 ? blockIdx.x * G + group : blockIdx.x / (uint32_t)A.segments;  // (a row by a wave has one segment)
+  const int64_t row = A.row0 + unit;
   if (row >= A.rows) return;  // (G > 1 only: a wave for itself)
-  const int seg = A.segments == 1 ? 0 : (int)(unit - row * A.segments);
+  const int seg = G > 1 ? 0 : (int)(blockIdx.x - unit * (uint32_t)A.segments);
   const int j0 = seg * A.per_segment, n = min(A.per_segment, A.classes - j0);
   const T* x = static_cast<const T*>(A.x) + row * A.stride + j0;
   T* dx = static_cast<T*>(A.dx) + row * (int64_t)A.classes + j0;
@@ -857,29 +859,37 @@ Cut bwd_cut(int32_t classes, int32_t type) {
   const int32_t per = 256 * kU * (type == VITTA_SCORES_F32 ? 4 : 8);
   return classes <= kWaveGrad || classes <= per ? Cut{1, classes} : Cut{(int32_t)(((int64_t)classes + per - 1) / per), per};
 }
-// sizes a launch does not take: more workgroups than a grid has, rows that no 64 segments of kTailSegment hold
-bool too_large(int64_t rows, int32_t classes, int32_t type, bool top) {
-  if (classes > kMaxSegments * kTailSegment || rows > 0x7fffffff) return true;
-  return rows * (int64_t)fwd_cut(rows, classes, type, top).segments > 0x7fffffff || rows * (int64_t)bwd_cut(classes, type).segments > 0x7fffffff;
+// Rows of one launch: its threads stay below 2^31 (a grid of 2^32 and more is refused); a multiple of 4, the rows of a workgroup by waves.
+int64_t launch_rows(int32_t segments, int threads) {
+  const int64_t n = (int64_t)0x7fffffff / ((int64_t)segments * threads) & ~(int64_t)3;
+  return n < 4 ? 4 : n;
 }
+
+// rows that no 64 segments of kTailSegment classes hold
+bool too_large(int64_t rows, int32_t classes) { return classes > kMaxSegments * kTailSegment || rows > 0x7fffffff; }
 
 template <typename T, int MODE, bool ENT, bool TOP>
 int launch_fwd(FwdArgs a, void* ws, uint32_t* tickets, hipStream_t st) {
   const Cut cut = fwd_cut(a.rows, a.classes, Pack<T>::N == 4 ? VITTA_SCORES_F32 : VITTA_SCORES_BF16, TOP);
   a.segments = cut.segments, a.per_segment = cut.per_segment;
   const size_t bits = MODE == kDistillTail ? ((size_t)(cut.per_segment + 16 + 31) / 32 + 1) * 4 : 0;
-  if (wave_rows(a.rows, a.classes, TOP)) {
-    VITTA_LAUNCH((scores_kernel<T, 1, MODE, ENT, TOP>), dim3((unsigned)((a.rows + 3) / 4)), dim3(256), 4 * bits, st, a);
-    return VITTA_OK;
-  }
+  constexpr int NW = waves_of(TOP);
+  const bool waves = wave_rows(a.rows, a.classes, TOP);
   if (cut.segments > 1) {
     a.part = static_cast<float4*>(ws);
     a.keys = reinterpret_cast<uint64_t*>(a.part + a.rows * cut.segments);
     a.tickets = tickets;
   }
-  constexpr int NW = waves_of(TOP);
-  VITTA_LAUNCH((scores_kernel<T, NW, MODE, ENT, TOP>), dim3((unsigned)(a.rows * cut.segments)), dim3(NW * 64), bits, st, a);
-  if (cut.segments > 1 && !tickets) VITTA_LAUNCH((scores_join_kernel<T, MODE, TOP>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  const int64_t most = launch_rows(cut.segments, waves ? 64 : NW * 64);
+  for (a.row0 = 0; a.row0 < a.rows; a.row0 += most) {
+    const int64_t rows = a.rows - a.row0 < most ? a.rows - a.row0 : most;
+    if (waves) {
+      VITTA_LAUNCH((scores_kernel<T, 1, MODE, ENT, TOP>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 4 * bits, st, a);
+      continue;
+    }
+    VITTA_LAUNCH((scores_kernel<T, NW, MODE, ENT, TOP>), dim3((unsigned)(rows * cut.segments)), dim3(NW * 64), bits, st, a);
+    if (cut.segments > 1 && !tickets) VITTA_LAUNCH((scores_join_kernel<T, MODE, TOP>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  }
   return VITTA_OK;
 }
 
@@ -895,12 +905,16 @@ template <typename T, bool DISTILL, bool ENT>
 int launch_bwd(BwdArgs a, hipStream_t st) {
   const Cut cut = bwd_cut(a.classes, Pack<T>::N == 4 ? VITTA_SCORES_F32 : VITTA_SCORES_BF16);
   a.segments = cut.segments, a.per_segment = cut.per_segment;
-  const int64_t units = a.rows * cut.segments;
   // A gradient of 512 MiB and more is streamed past the 256 MiB cache (2048 x 131072 bfloat16 188 -> 180 us); a smaller one stays in it, for the
   // store itself and for who reads it next (1024 x 131072 87 -> 91 us, 1024 x 50021 floats 58 -> 75 if it were streamed).
   a.stream_out = a.rows * a.classes * (int64_t)sizeof(T) >= (512ll << 20);
-  if (a.classes <= kWaveGrad) VITTA_LAUNCH((scores_grad_kernel<T, 64, DISTILL, ENT>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, st, a);
-  else VITTA_LAUNCH((scores_grad_kernel<T, 256, DISTILL, ENT>), dim3((unsigned)units), dim3(256), 0, st, a);
+  const bool waves = a.classes <= kWaveGrad;
+  const int64_t most = launch_rows(cut.segments, waves ? 64 : 256);
+  for (a.row0 = 0; a.row0 < a.rows; a.row0 += most) {
+    const int64_t rows = a.rows - a.row0 < most ? a.rows - a.row0 : most;
+    if (waves) VITTA_LAUNCH((scores_grad_kernel<T, 64, DISTILL, ENT>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    else VITTA_LAUNCH((scores_grad_kernel<T, 256, DISTILL, ENT>), dim3((unsigned)(rows * cut.segments)), dim3(256), 0, st, a);
+  }
   return VITTA_OK;
 }
 
@@ -917,7 +931,7 @@ int launch_bwd(int32_t type, const BwdArgs& a, void* stream) {
 extern "C" {
 
 size_t vitta_scores_workspace_bytes(int64_t rows, int32_t classes, int32_t dtype, int32_t top) {
-  if (rows <= 0 || classes <= 0 || top < 0 || top > VITTA_SCORES_MAX_TOP || too_large(rows, classes, dtype, top > 0)) return 0;
+  if (rows <= 0 || classes <= 0 || top < 0 || top > VITTA_SCORES_MAX_TOP || too_large(rows, classes)) return 0;
   const int64_t s = fwd_cut(rows, classes, dtype, top > 0).segments;
   return s == 1 ? 0 : (size_t)rows * s * (16 + 8 * (size_t)top);
 }
@@ -930,7 +944,7 @@ int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32
   if (top < 0 || top > VITTA_SCORES_MAX_TOP || top > classes || (top > 0 && (!d_top_logprob || !d_top_index))) return VITTA_ERR_INVALID_ARG;
   if (!d_labels != !d_logprob || (!d_logprob && !d_entropy && !d_lse && top == 0)) return VITTA_ERR_INVALID_ARG;
   if (d_stats && bad_stats(d_stats)) return VITTA_ERR_INVALID_ARG;
-  if (too_large(rows, classes, dtype, top > 0)) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   const size_t need = vitta_scores_workspace_bytes(rows, classes, dtype, top);
   if (workspace_bytes < need || (need && bad_stats(d_workspace))) return VITTA_ERR_WORKSPACE;
   FwdArgs a{};
@@ -948,7 +962,7 @@ int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32
                              void* stream) {
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature) || bad_stats(d_stats) || bad_out(d_dx, dtype)) return VITTA_ERR_INVALID_ARG;
   if ((d_glogprob && !d_labels) || (d_gtop && (!d_top_index || top <= 0 || top > VITTA_SCORES_MAX_TOP))) return VITTA_ERR_INVALID_ARG;
-  if (too_large(rows, classes, dtype, false)) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   BwdArgs a{};
   a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.labels = d_labels, a.ignore = ignore_index, a.top = top, a.top_index = d_top_index;
@@ -963,7 +977,7 @@ int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t 
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || !d_value || !d_loss || bad_stats(d_stats) || !d_q || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
   if (value_dtype < VITTA_SCORES_F32 || value_dtype > VITTA_SCORES_F16) return VITTA_ERR_INVALID_ARG;
-  if (too_large(rows, classes, dtype, false)) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   const size_t need = vitta_scores_workspace_bytes(rows, classes, dtype, 0);
   if (workspace_bytes < need || (need && bad_stats(d_workspace))) return VITTA_ERR_WORKSPACE;
   FwdArgs a{};
@@ -978,7 +992,7 @@ int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t 
                           int64_t g_stride, void* d_dx, void* stream) {
   if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || bad_stats(d_stats) || !d_q || !d_g || bad_out(d_dx, dtype) || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
-  if (too_large(rows, classes, dtype, false)) return VITTA_ERR_UNSUPPORTED;
+  if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   BwdArgs a{};
   a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
   a.stats = d_stats, a.index = d_index, a.list = list, a.q = d_q, a.g = d_g, a.s_g = g_stride;

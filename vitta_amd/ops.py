@@ -317,7 +317,8 @@ _label_logprobs_again = once_differentiable(_label_logprobs_grad)  # (under crea
 def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, temperature=1.0, ignore_index=-100):
     """Log probability of given labels, entropy and best alternatives of rows of class scores, read once.
 
-    logits (..., V) float32 / bfloat16 / float16 (rows may be cut from a wider matrix); labels (...) int64 or int32, or None.
+    logits (..., V) float32 / bfloat16 / float16 (rows may be cut from a wider matrix; V at most 2 ** 24); labels (...) int64 or int32, or
+    None.
     Returns a LabelLogprobs of float32 tensors shaped (...): with z = logits / temperature,
       logprob       z[label] - lse; 0 where label == ignore_index; NaN where the label is no class (None without labels)
       entropy       -sum p log p, p = softmax(z) (None with entropy=False)
@@ -386,7 +387,7 @@ _top_distill_again = once_differentiable(_top_distill_grad)
 def top_distill(student_logits, teacher_index, teacher_value, *, temperature=1.0, tail=False):
     """KL divergence of a student from a teacher of whom only a list of best classes is kept, a float32 loss per row.
 
-    student_logits (..., V) float32 / bfloat16 / float16; teacher_index (..., K) int64 or int32 and teacher_value (..., K) float32 /
+    student_logits (..., V) float32 / bfloat16 / float16, V at most 2 ** 24; teacher_index (..., K) int64 or int32 and teacher_value (..., K) float32 /
     bfloat16 / float16, K at most 256, without gradient; an index that is no class (-1, as `label_logprobs` gives) is padding, and a
     row of padding only has loss 0 and gradient 0.  p = softmax(student_logits / temperature) over all V classes, and
       tail=False  q = softmax(teacher_value / temperature) over the list:  sum q (log q - log p)
