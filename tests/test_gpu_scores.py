@@ -428,6 +428,56 @@ def test_teacher_list_from_the_readout_trains_a_student():
             assert (best.top_index[:, 15:] == -1).all()
 
 
+@pytest.mark.parametrize("rows,classes,dtype", [(2, 600001, torch.float32), (520, 300001, torch.bfloat16), (1, 2 ** 24, torch.float16)])
+def test_very_long_rows(rows, classes, dtype):
+    """More classes than one workgroup's membership bits hold, few rows and more than have tickets; the largest vocabulary."""
+    from vitta_amd import _lib, ops
+    gen = torch.Generator(device=DEV).manual_seed(classes)
+    dx = torch.empty(rows, classes, dtype=dtype, device=DEV).normal_(0, 2, generator=gen)
+    index, value = _list(1, classes, 33, 5, True)
+    index, value = (index + torch.arange(rows)[:, None]) % classes, value.expand(rows, 33).contiguous()
+    index[0, -2:] = torch.tensor([0, classes - 1])
+    labels = torch.arange(rows) * 7
+    leaf = dx.requires_grad_()
+    o = ops.label_logprobs(leaf, labels.to(DEV), top=64, lse=True)
+    loss = ops.top_distill(leaf, index.to(DEV), value.to(DEV), tail=True)
+    (g1,) = torch.autograd.grad(o.entropy, leaf, torch.ones(rows, device=DEV))
+    (g2,) = torch.autograd.grad(loss, leaf, torch.ones(rows, device=DEV))
+    for r in {0, rows // 2, rows - 1}:
+        x = dx[r:r + 1].detach().cpu()
+        _check_readout(ops.LabelLogprobs(*[t[r:r + 1].detach() for t in o]), x, labels[r:r + 1], 64, 1.0)
+        want, bound = O.readout_grad(x, labels[r:r + 1], 64, 1.0, None, torch.ones(1))
+        _check_grad(g1[r:r + 1], want, bound, dtype)
+        want, grad_want, b_loss, b_grad = O.distill(x, index[r:r + 1], value[r:r + 1], 1.0, True)
+        _close(loss[r:r + 1], want, b_loss, "loss")
+        _check_grad(g2[r:r + 1], grad_want, b_grad, dtype)
+    if classes == 2 ** 24:
+        with pytest.raises(_lib.VittaHipError, match="unsupported|nsupported"):
+            ops.label_logprobs(torch.zeros(1, classes + 1, dtype=dtype, device=DEV))
+
+
+def test_gradients_of_no_rows():
+    from vitta_amd import ops
+    leaf = torch.zeros(0, 3, 9, device=DEV, requires_grad=True)
+    o = ops.label_logprobs(leaf, torch.zeros(0, 3, dtype=torch.long, device=DEV), top=2)
+    loss = ops.top_distill(leaf, torch.zeros(0, 3, 4, dtype=torch.long, device=DEV), torch.zeros(0, 3, 4, device=DEV))
+    assert o.top_index.shape == (0, 3, 2) and loss.shape == (0, 3)
+    (grad,) = torch.autograd.grad((o.logprob.sum() + o.entropy.sum() + loss.sum()), leaf)
+    assert grad.shape == leaf.shape
+
+
+def test_modified_scores_are_noticed():
+    """The backward reads the scores again: changed in place in between, they are an error and not a wrong gradient."""
+    from vitta_amd import ops
+    x = torch.randn(3, 20, device=DEV)
+    leaf = x.clone().requires_grad_()
+    y = leaf * 1.0
+    o = ops.label_logprobs(y)
+    y.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.entropy.sum().backward()
+
+
 def test_far_offsets():
     """Rows that begin beyond 2^31 elements."""
     from vitta_amd import ops
