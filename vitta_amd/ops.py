@@ -270,45 +270,46 @@ def _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_inde
 
 
 class _LabelLogprobs(torch.autograd.Function):
+    """how: the arguments of _label_logprobs behind m.  Only the results that were asked pass through autograd."""
+
     @staticmethod
-    def forward(ctx, m, lead, labels, top, entropy, lse, temperature, ignore_index):
+    def forward(ctx, m, how):
         stats = m.new_empty((m.shape[0], 4), dtype=torch.float32)
-        out = _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_index, stats)
-        ctx.save_for_backward(m, labels, out[4], stats)
-        ctx.how = (top, temperature, ignore_index)
-        if top:
+        out = _label_logprobs(m, *how, stats)
+        ctx.save_for_backward(m, how[1], out[4], stats)
+        ctx.how = how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
+        if how[2]:
             ctx.mark_non_differentiable(out[4])
         ctx.set_materialize_grads(False)
-        return out
+        return tuple([t for t in out if t is not None])
 
     @staticmethod
     def backward(ctx, *g):
         return (_label_logprobs_again if torch.is_grad_enabled() else _label_logprobs_grad)(ctx, *g)
 
 
-def _label_logprobs_grad(ctx, g_logprob, g_entropy, g_lse, g_top, _):
+def _label_logprobs_grad(ctx, *upstream):
     m, labels, top_index, stats = ctx.saved_tensors
-    top, temperature, ignore_index = ctx.how
+    top, temperature, ignore_index, asked = ctx.how
     rows, classes = m.shape
     dx = m.new_empty((rows, classes))
     if rows:
-        a = b = c = d = e = y = None
-        sa = sb = sc = 0
-        if g_logprob is not None:
-            g_logprob, sa = _row_gradient(g_logprob)
-            a, y = g_logprob.data_ptr(), labels.data_ptr()
-        if g_entropy is not None:
-            g_entropy, sb = _row_gradient(g_entropy)
-            b = g_entropy.data_ptr()
-        if g_lse is not None:
-            g_lse, sc = _row_gradient(g_lse)
-            c = g_lse.data_ptr()
-        if g_top is not None:
-            g_top = g_top.contiguous()
-            d, e = g_top.data_ptr(), top_index.data_ptr()
-        _call("vitta_label_logprobs_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, y,
-              ignore_index, top, e, stats.data_ptr(), a, sa, b, sb, c, sc, d, dx.data_ptr())
-    return dx, None, None, None, None, None, None, None
+        at, stride, index, label = [None] * 4, [0] * 3, None, None
+        keep = []  # (dense copies live until the launch is issued)
+        for i, g in zip(asked, upstream):
+            if g is None:
+                continue
+            if i == 3:
+                g, index = g.contiguous(), top_index.data_ptr()
+            else:
+                g, stride[i] = _row_gradient(g)
+                if i == 0:
+                    label = labels.data_ptr()
+            keep.append(g)
+            at[i] = g.data_ptr()
+        _call("vitta_label_logprobs_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, label,
+              ignore_index, top, index, stats.data_ptr(), at[0], stride[0], at[1], stride[1], at[2], stride[2], at[3], dx.data_ptr())
+    return dx, None
 
 
 _label_logprobs_again = once_differentiable(_label_logprobs_grad)  # (under create_graph: a second derivative is refused, not taken as 0)
@@ -335,9 +336,12 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
     lead = logits.shape[:-1]
     if labels is not None:
         labels = _score_side(labels, "labels", logits, lead, (torch.int64, torch.int32))
-    if m.requires_grad and torch.is_grad_enabled():
-        return LabelLogprobs(*_LabelLogprobs.apply(m, lead, labels, int(top), entropy, lse, float(temperature), int(ignore_index)))
-    return LabelLogprobs(*_label_logprobs(m, lead, labels, int(top), entropy, lse, float(temperature), int(ignore_index), None))
+    how = lead, labels, int(top), entropy, lse, float(temperature), int(ignore_index)
+    if not (m.requires_grad and torch.is_grad_enabled()):
+        return LabelLogprobs(*_label_logprobs(m, *how, None))
+    out = iter(_LabelLogprobs.apply(m, how))
+    return LabelLogprobs(next(out) if labels is not None else None, next(out) if entropy else None, next(out) if lse else None,
+                         next(out) if top else None, next(out) if top else None)
 
 
 def _top_distill(m, lead, index, value, temperature, tail):
@@ -357,11 +361,13 @@ def _top_distill(m, lead, index, value, temperature, tail):
 
 
 class _TopDistill(torch.autograd.Function):
+    """how: the arguments of _top_distill behind m"""
+
     @staticmethod
-    def forward(ctx, m, lead, index, value, temperature, tail):
-        loss, side = _top_distill(m, lead, index, value, temperature, tail)
-        ctx.save_for_backward(m, index, side)
-        ctx.temperature = temperature
+    def forward(ctx, m, how):
+        loss, side = _top_distill(m, *how)
+        ctx.save_for_backward(m, how[1], side)
+        ctx.temperature = how[3]
         return loss
 
     @staticmethod
@@ -374,11 +380,11 @@ def _top_distill_grad(ctx, g):
     rows, classes = m.shape
     dx = m.new_empty((rows, classes))
     if rows:
-        g, sg = _row_gradient(g)
+        g, stride = _row_gradient(g)
         stats = side.data_ptr()
         _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), ctx.temperature,
-              index.data_ptr(), index.shape[-1], stats, stats + 16 * rows, g.data_ptr(), sg, dx.data_ptr())
-    return dx, None, None, None, None, None
+              index.data_ptr(), index.shape[-1], stats, stats + 16 * rows, g.data_ptr(), stride, dx.data_ptr())
+    return dx, None
 
 
 _top_distill_again = once_differentiable(_top_distill_grad)
@@ -404,9 +410,10 @@ def top_distill(student_logits, teacher_index, teacher_value, *, temperature=1.0
     shape = lead + teacher_index.shape[-1:]
     index = _score_side(teacher_index, "teacher_index", student_logits, shape, (torch.int64, torch.int32))
     value = _score_side(teacher_value, "teacher_value", student_logits, shape, _SCORE_TYPES)
+    how = lead, index, value, float(temperature), bool(tail)
     if m.requires_grad and torch.is_grad_enabled():
-        return _TopDistill.apply(m, lead, index, value, float(temperature), bool(tail))
-    return _top_distill(m, lead, index, value, float(temperature), bool(tail))[0]
+        return _TopDistill.apply(m, how)
+    return _top_distill(m, *how)[0]
 
 
 # ------------------------------------------------------------------------------------------------
