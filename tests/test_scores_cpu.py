@@ -128,6 +128,12 @@ def test_distillation_gradient_refusals(bad):
     assert _lib.lib().vitta_top_distill_bwd(*a.values(), None) == -1
 
 
+def test_library_is_built_without_packed_float32_instructions():
+    from vitta_amd import build
+    flags = " ".join(build.CFLAGS)
+    assert "-Xclang -target-feature -Xclang -packed-fp32-ops" in flags and "-ffast-math" not in flags
+
+
 def test_workspace_is_plain_host_arithmetic():
     f = _lib.lib().vitta_scores_workspace_bytes
     assert isinstance(f(1, 131072, 1, 64), int) and f(4096, 101, 0, 5) >= 0 and ctypes.sizeof(ctypes.c_size_t) == 8
