@@ -872,8 +872,9 @@ int vitta_frames_cv2_resize(const uint8_t* d_frames, int32_t n_frames, int32_t i
 
 /* --------------------------------------------------------------------------
  * Rows of class scores (logits): what they say of a label, how sure they are, and a loss against another model's answer.
- *   d_x     [rows][row_stride] scores, classes of them used per row (row_stride in elements, any >= 0); dtype one of the
- *           VITTA_SCORES_* below, element aligned; at most 2^24 classes and 2^31 - 1 rows;  z = x / temperature,  p = softmax(z)
+ *   d_x     scores, `classes` of them in a row; row r begins at element (r / inner_rows) outer_stride + (r % inner_rows) row_stride (any
+ *           strides >= 0; a matrix: inner_rows = rows), dtype one of the VITTA_SCORES_* below, element aligned; at most 2^24 classes
+ *           and 2^31 - 1 rows;  z = x / temperature,  p = softmax(z)
  * vitta_label_logprobs_fwd, any of the outputs may be NULL:
  *   d_logprob [rows]      z_y - lse of label y = d_labels[row]; 0 where y == ignore_index, NaN where y is no class (nothing is read)
  *   d_entropy [rows]      -sum p log p        d_lse [rows]  log sum exp z
@@ -901,19 +902,23 @@ int vitta_frames_cv2_resize(const uint8_t* d_frames, int32_t n_frames, int32_t i
 #define VITTA_SCORES_MAX_TOP 64
 #define VITTA_SCORES_MAX_LIST 256
 size_t vitta_scores_workspace_bytes(int64_t rows, int32_t classes, int32_t dtype, int32_t top);
-int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, int64_t inner_rows,
+                             int64_t outer_stride, float temperature,
                              const int64_t* d_labels, int64_t ignore_index, int32_t top, float* d_logprob, float* d_entropy,
                              float* d_lse, float* d_top_logprob, int64_t* d_top_index, float* d_stats, void* d_workspace,
                              size_t workspace_bytes, uint32_t* d_tickets, void* stream);
-int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, int64_t inner_rows,
+                             int64_t outer_stride, float temperature,
                              const int64_t* d_labels, int64_t ignore_index, int32_t top, const int64_t* d_top_index,
                              const float* d_stats, const float* d_glogprob, int64_t glogprob_stride, const float* d_gentropy,
                              int64_t gentropy_stride, const float* d_glse, int64_t glse_stride, const float* d_gtop, void* d_dx,
                              void* stream);
-int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, int64_t inner_rows,
+                             int64_t outer_stride, float temperature,
                           const int64_t* d_index, const void* d_value, int32_t value_dtype, int32_t list, int32_t tail, float* d_loss,
                           float* d_stats, float* d_q, void* d_workspace, size_t workspace_bytes, uint32_t* d_tickets, void* stream);
-int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, int64_t inner_rows,
+                             int64_t outer_stride, float temperature,
                           const int64_t* d_index, int32_t list, const float* d_stats, const float* d_q, const float* d_g,
                           int64_t g_stride, void* d_dx, void* stream);
 

@@ -104,6 +104,41 @@ def test_readout_leading_dimensions_and_empty_ones():
         assert torch.equal(a, b) and torch.equal(c, a[:1].expand_as(c))
 
 
+@pytest.mark.parametrize("classes", [37, 5001, 40003])
+def test_rows_cut_from_sequences(classes):
+    """Shifted sequences, transposed leading dimensions and broadcast ones, without a copy of the scores where two strides say it all."""
+    from vitta_amd import ops
+    whole = (torch.randn(3, 6, classes + 2, generator=torch.Generator().manual_seed(classes)) * 2).bfloat16()
+    on = whole.to(DEV)
+    labels = torch.randint(classes, (3, 5), generator=torch.Generator().manual_seed(1))
+    for make in (lambda t: t[:, :-1, :classes], lambda t: t[:, 1:, 2:].transpose(0, 1), lambda t: t[:, :1, 1:classes + 1].expand(-1, 5, -1),
+                 lambda t: t[:, ::2, :classes].unsqueeze(1)):
+        x, leaf = make(whole), on.clone().requires_grad_()
+        cut = make(leaf)
+        y = labels.t().contiguous() if x.shape[:2] == (5, 3) else labels if x.shape[:2] == (3, 5) else labels[:, None, :3].contiguous()
+        assert ops._score_rows(cut, "x", 1.0)[0] is cut
+        o = ops.label_logprobs(cut, y.to(DEV), top=3, lse=True)
+        flat = x.reshape(-1, classes)
+        assert o.logprob.shape == x.shape[:-1] and o.top_index.shape == x.shape[:-1] + (3,)
+        _check_readout(ops.LabelLogprobs(*[t.flatten(0, x.dim() - 2) for t in o]), flat, y.reshape(-1), 3, 1.0)
+        up = torch.randn(flat.shape[0], generator=torch.Generator().manual_seed(2))
+        index, value = _list(flat.shape[0], classes, 4, 3, True)
+        lead = x.shape[:-1] + (4,)
+        loss = ops.top_distill(cut, index.view(lead).to(DEV), value.view(lead).to(DEV), tail=True)
+        want, grad_want, b_loss, b_grad = O.distill(flat, index, value, 1.0, True)
+        _close(loss.flatten(), want, b_loss, "loss")
+        (grad,) = torch.autograd.grad((o.entropy, loss), cut, (up.view(x.shape[:-1]).to(DEV), torch.ones(x.shape[:-1], device=DEV)), retain_graph=True)
+        want, bound = O.readout_grad(flat, None, 0, 1.0, None, up)
+        # two gradients, each rounded to bfloat16, and their sum
+        _check_grad(grad.reshape(-1, classes), want + grad_want, bound + b_grad + 2 * O.half_step(torch.bfloat16) * (want.abs() + grad_want.abs()), torch.bfloat16)
+        (grad,) = torch.autograd.grad(o.logprob.sum(), leaf)
+        assert grad.shape == whole.shape
+    deep = on.view(3, 2, 3, classes + 2)[:, :, :2, :classes]  # three groups: a copy, the same answers
+    a = ops.label_logprobs(deep.transpose(0, 2), top=2)
+    b = ops.label_logprobs(deep.transpose(0, 2).contiguous(), top=2)
+    assert torch.equal(a.entropy, b.entropy) and torch.equal(a.top_index, b.top_index)
+
+
 ROWS = ["-inf", "one", "two", "lowest", "some lowest", "equal", "zeros", "rising", "falling", "nan", "nan last", "inf", "huge"]
 
 

@@ -73,14 +73,14 @@ def test_operators_refuse_host_tensors():
 
 
 def _fwd(**kw):
-    a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, t=1.0, labels=4096, ignore=-100, top=0, logprob=4096, entropy=None, lse=4096,
+    a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, inner=2, outer=0, t=1.0, labels=4096, ignore=-100, top=0, logprob=4096, entropy=None, lse=4096,
              top_logprob=None, top_index=None, stats=None, ws=None, ws_bytes=1 << 40, tickets=None)
     a.update(kw)
     return _lib.lib().vitta_label_logprobs_fwd(*a.values(), None)
 
 
 # every call below is refused before any launch: no pointer is read
-@pytest.mark.parametrize("bad", [dict(x=None), dict(dtype=3), dict(dtype=-1), dict(rows=0), dict(rows=-1), dict(classes=0), dict(stride=-1),
+@pytest.mark.parametrize("bad", [dict(x=None), dict(dtype=3), dict(dtype=-1), dict(rows=0), dict(rows=-1), dict(classes=0), dict(stride=-1), dict(inner=0), dict(inner=-3), dict(outer=-1),
                                  dict(t=0.0), dict(t=-1.0), dict(t=math.nan), dict(t=math.inf), dict(x=4097), dict(x=4098), dict(top=-1),
                                  dict(top=11), dict(top=65, classes=100, top_logprob=4096, top_index=4096), dict(top=3),
                                  dict(top=3, top_logprob=4096), dict(labels=None), dict(logprob=None), dict(stats=4104),
@@ -89,13 +89,39 @@ def test_readout_refusals(bad):
     assert _fwd(**bad) == -1
 
 
+def test_layouts_of_rows():
+    """What _row_layout says of a layout names the rows' addresses, over random views; None only where two strides do not do."""
+    gen = torch.Generator().manual_seed(1)
+    said = 0
+    for _ in range(400):
+        n = int(torch.randint(1, 5, (1,), generator=gen))
+        x = torch.arange(4 * 5 * 3 * 6).view(4, 5, 3, 6)
+        for d in range(3):
+            lo = int(torch.randint(0, 2, (1,), generator=gen))
+            hi = x.shape[d] - int(torch.randint(0, 2, (1,), generator=gen))
+            x = x.narrow(d, lo, max(1, hi - lo))
+        x = x[..., :4] if n == 1 else x.transpose(0, 1) if n == 2 else x[:, :1].expand(-1, 5, -1, -1) if n == 3 else x[:, 0]
+        got = ops._row_layout(x.shape, x.stride())
+        if got is None:
+            continue
+        said += 1
+        stride, inner, outer = got
+        base = x.storage_offset()
+        rows = x.numel() // x.shape[-1]
+        want = x.reshape(rows, -1)[:, 0]
+        have = torch.tensor([base + (r // inner) * outer + (r % inner) * stride for r in range(rows)])
+        assert torch.equal(want, have)
+    assert said > 200
+    assert ops._row_layout((3, 4), (1, 3)) is None and ops._row_layout((2, 2, 2, 5), (100, 30, 7, 1)) is None
+
+
 def test_sizes_beyond_a_launch_are_refused():
     assert _fwd(rows=1 << 40) == -4
     assert _fwd(classes=(1 << 24) + 1, stride=1 << 25) == -4
 
 
 def _bwd(**kw):
-    a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, t=1.0, labels=4096, ignore=-100, top=0, top_index=None, stats=4096, g1=4096,
+    a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, inner=2, outer=0, t=1.0, labels=4096, ignore=-100, top=0, top_index=None, stats=4096, g1=4096,
              s1=1, g2=None, s2=0, g3=None, s3=0, gtop=None, dx=4096)
     a.update(kw)
     return _lib.lib().vitta_label_logprobs_bwd(*a.values(), None)
@@ -108,7 +134,7 @@ def test_readout_gradient_refusals(bad):
 
 
 def _distil(**kw):
-    a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, t=1.0, index=4096, value=4096, value_dtype=0, list=3, tail=0, loss=4096,
+    a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, inner=2, outer=0, t=1.0, index=4096, value=4096, value_dtype=0, list=3, tail=0, loss=4096,
              stats=4096, q=4096, ws=None, ws_bytes=1 << 40, tickets=None)
     a.update(kw)
     return _lib.lib().vitta_top_distill_fwd(*a.values(), None)
@@ -123,7 +149,7 @@ def test_distillation_refusals(bad):
 @pytest.mark.parametrize("bad", [dict(x=None), dict(index=None), dict(stats=None), dict(stats=4104), dict(q=None), dict(g=None), dict(dx=None),
                                  dict(dx=4097), dict(list=0), dict(list=257)])
 def test_distillation_gradient_refusals(bad):
-    a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, t=1.0, index=4096, list=3, stats=4096, q=4096, g=4096, s_g=1, dx=4096)
+    a = dict(x=4096, dtype=0, rows=2, classes=10, stride=10, inner=2, outer=0, t=1.0, index=4096, list=3, stats=4096, q=4096, g=4096, s_g=1, dx=4096)
     a.update(bad)
     assert _lib.lib().vitta_top_distill_bwd(*a.values(), None) == -1
 

@@ -101,11 +101,11 @@ SIGNATURES = {
                                            _p, _p, _p, _p, _p, _p, _p]),
     "vitta_stat_align_bwd_f32": (C.c_int, [_p, _p, _p, _i64, _i32, _i64, _i32, _p, _p, _p, _p, _p]),
     "vitta_scores_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
-    "vitta_label_logprobs_fwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _f32, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _p]),
-    "vitta_label_logprobs_bwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _f32, _p, _i64, _i32, _p, _p, _p, _i64, _p, _i64, _p, _i64,
+    "vitta_label_logprobs_fwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _i64, _i64, _f32, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _p]),
+    "vitta_label_logprobs_bwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _i64, _i64, _f32, _p, _i64, _i32, _p, _p, _p, _i64, _p, _i64, _p, _i64,
                                            _p, _p, _p]),
-    "vitta_top_distill_fwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _f32, _p, _p, _i32, _i32, _i32, _p, _p, _p, _p, _sz, _p, _p]),
-    "vitta_top_distill_bwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _f32, _p, _i32, _p, _p, _p, _i64, _p, _p]),
+    "vitta_top_distill_fwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _i64, _i64, _f32, _p, _p, _i32, _i32, _i32, _p, _p, _p, _p, _sz, _p, _p]),
+    "vitta_top_distill_bwd": (C.c_int, [_p, _i32, _i64, _i32, _i64, _i64, _i64, _f32, _p, _i32, _p, _p, _p, _i64, _p, _p]),
     "vitta_pred_consis_f32": (C.c_int, [_p, _i32, _i32, _i32, _p, _p, _p]),
     "vitta_tam_pool_f32": (C.c_int, [_p, _i32, _i32, _i32, _i32, _p, _p]),
     "vitta_tam_agg_fwd_f32": (C.c_int, [_p, _p, _p, _i32, _i32, _i32, _i32, _p, _p]),

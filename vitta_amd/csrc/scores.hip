@@ -257,7 +257,8 @@ struct Best {
 // ---- arguments ---------------------------------------------------------------------------------------------------------------------
 struct FwdArgs {
   const void* x;
-  int64_t rows, stride, row0;  // row0: the launch's first row
+  int64_t rows, stride, outer, row0;  // row0: the launch's first row
+  uint32_t inner;                     // rows at `stride` from one another, groups of them at `outer`
   int32_t classes, segments, per_segment;
   float c, inv_t;
   float* stats;
@@ -276,6 +277,11 @@ struct FwdArgs {
   int32_t value_type, list;
   float *loss, *q;
 };
+
+template <typename T, class Args> __device__ __forceinline__ const T* row_of(const Args& A, int64_t row) {
+  const int64_t group = A.inner < A.rows ? (uint32_t)row / A.inner : 0;  // (rows < 2^31)
+  return static_cast<const T*>(A.x) + group * A.outer + (row - group * A.inner) * A.stride;
+}
 
 enum Mode { kReadout, kDistill, kDistillTail };
 
@@ -405,7 +411,7 @@ template <typename V> __device__ __forceinline__ V get(const V* p) { return __hi
 // NW waves merge the lists (64 keys at a time, four loads ahead), the first one the sums
 template <typename T, int MODE, bool TOP, int NW>
 __device__ void join_segments(const FwdArgs& A, int64_t row, uint64_t* lists, int lane, int wave) {
-  const T* x = static_cast<const T*>(A.x) + row * A.stride;
+  const T* x = row_of<T>(A, row);
   Best best{0, false};
   if (TOP) {
     const int all = A.segments * A.top;
@@ -457,7 +463,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
     row = A.row0 + at;
     seg = (int)(blockIdx.x - at * (uint32_t)A.segments);
   }
-  const T* whole = static_cast<const T*>(A.x) + row * A.stride;
+  const T* whole = row_of<T>(A, row);
   const int j0 = seg * A.per_segment, n = min(A.per_segment, A.classes - j0);
   const T* x = whole + j0;
   const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
@@ -689,7 +695,8 @@ __global__ __launch_bounds__(256) void scores_join_kernel(FwdArgs A) {
 struct BwdArgs {
   const void* x;
   void* dx;
-  int64_t rows, stride, row0;
+  int64_t rows, stride, outer, row0;
+  uint32_t inner;
   int32_t classes, segments, per_segment;
   float c, inv_t;
   const float* stats;
@@ -722,7 +729,7 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
   if (row >= A.rows) return;  // (G > 1 only: a wave for itself)
   const int seg = G > 1 ? 0 : (int)(blockIdx.x - unit * (uint32_t)A.segments);
   const int j0 = seg * A.per_segment, n = min(A.per_segment, A.classes - j0);
-  const T* x = static_cast<const T*>(A.x) + row * A.stride + j0;
+  const T* x = row_of<T>(A, row) + j0;
   T* dx = static_cast<T*>(A.dx) + row * (int64_t)A.classes + j0;
   const int head = min(n, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
   const int nv = (n - head) / N, body = head + nv * N;
@@ -824,8 +831,8 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
 bool bad_stats(const void* p) { return !p || (reinterpret_cast<uintptr_t>(p) & 15u); }
 bool bad_out(const void* p, int32_t type) { return !p || reinterpret_cast<uintptr_t>(p) % (type == VITTA_SCORES_F32 ? 4 : 2); }
 
-bool bad_scores(const void* x, int32_t type, int64_t rows, int32_t classes, int64_t stride, float temperature) {
-  if (!x || type < VITTA_SCORES_F32 || type > VITTA_SCORES_F16 || rows <= 0 || classes <= 0 || stride < 0) return true;
+bool bad_scores(const void* x, int32_t type, int64_t rows, int32_t classes, int64_t stride, int64_t inner, int64_t outer, float temperature) {
+  if (!x || type < VITTA_SCORES_F32 || type > VITTA_SCORES_F16 || rows <= 0 || classes <= 0 || stride < 0 || inner <= 0 || outer < 0) return true;
   if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || temperature > 3e38f) return true;
   return reinterpret_cast<uintptr_t>(x) % (type == VITTA_SCORES_F32 ? 4 : 2) != 0;
 }
@@ -936,11 +943,12 @@ size_t vitta_scores_workspace_bytes(int64_t rows, int32_t classes, int32_t dtype
   return s == 1 ? 0 : (size_t)rows * s * (16 + 8 * (size_t)top);
 }
 
-int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, int64_t inner_rows,
+                             int64_t outer_stride, float temperature,
                              const int64_t* d_labels, int64_t ignore_index, int32_t top, float* d_logprob, float* d_entropy,
                              float* d_lse, float* d_top_logprob, int64_t* d_top_index, float* d_stats, void* d_workspace,
                              size_t workspace_bytes, uint32_t* d_tickets, void* stream) {
-  if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
+  if (bad_scores(d_x, dtype, rows, classes, row_stride, inner_rows, outer_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (top < 0 || top > VITTA_SCORES_MAX_TOP || top > classes || (top > 0 && (!d_top_logprob || !d_top_index))) return VITTA_ERR_INVALID_ARG;
   if (!d_labels != !d_logprob || (!d_logprob && !d_entropy && !d_lse && top == 0)) return VITTA_ERR_INVALID_ARG;
   if (d_stats && bad_stats(d_stats)) return VITTA_ERR_INVALID_ARG;
@@ -948,53 +956,60 @@ int vitta_label_logprobs_fwd(const void* d_x, int32_t dtype, int64_t rows, int32
   const size_t need = vitta_scores_workspace_bytes(rows, classes, dtype, top);
   if (workspace_bytes < need || (need && bad_stats(d_workspace))) return VITTA_ERR_WORKSPACE;
   FwdArgs a{};
-  a.x = d_x, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
+  a.x = d_x, a.rows = rows, a.stride = row_stride, a.outer = outer_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
+  a.inner = (uint32_t)(inner_rows < rows ? inner_rows : rows);
   a.stats = d_stats, a.labels = d_labels, a.ignore = ignore_index, a.top = top, a.logprob = d_logprob, a.entropy = d_entropy, a.lse = d_lse;
   a.top_logprob = d_top_logprob, a.top_index = d_top_index;
   if (d_entropy) return top ? launch_fwd<kReadout, true, true>(dtype, a, d_workspace, d_tickets, stream) : launch_fwd<kReadout, true, false>(dtype, a, d_workspace, d_tickets, stream);
   return top ? launch_fwd<kReadout, false, true>(dtype, a, d_workspace, d_tickets, stream) : launch_fwd<kReadout, false, false>(dtype, a, d_workspace, d_tickets, stream);
 }
 
-int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+int vitta_label_logprobs_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, int64_t inner_rows,
+                             int64_t outer_stride, float temperature,
                              const int64_t* d_labels, int64_t ignore_index, int32_t top, const int64_t* d_top_index,
                              const float* d_stats, const float* d_glogprob, int64_t glogprob_stride, const float* d_gentropy,
                              int64_t gentropy_stride, const float* d_glse, int64_t glse_stride, const float* d_gtop, void* d_dx,
                              void* stream) {
-  if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature) || bad_stats(d_stats) || bad_out(d_dx, dtype)) return VITTA_ERR_INVALID_ARG;
+  if (bad_scores(d_x, dtype, rows, classes, row_stride, inner_rows, outer_stride, temperature) || bad_stats(d_stats) || bad_out(d_dx, dtype)) return VITTA_ERR_INVALID_ARG;
   if ((d_glogprob && !d_labels) || (d_gtop && (!d_top_index || top <= 0 || top > VITTA_SCORES_MAX_TOP))) return VITTA_ERR_INVALID_ARG;
   if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   BwdArgs a{};
-  a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
+  a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.outer = outer_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
+  a.inner = (uint32_t)(inner_rows < rows ? inner_rows : rows);
   a.stats = d_stats, a.labels = d_labels, a.ignore = ignore_index, a.top = top, a.top_index = d_top_index;
   a.g_logprob = d_glogprob, a.g_entropy = d_gentropy, a.g_lse = d_glse, a.g_top = d_gtop;
   a.s_logprob = glogprob_stride, a.s_entropy = gentropy_stride, a.s_lse = glse_stride;
   return d_gentropy ? launch_bwd<false, true>(dtype, a, stream) : launch_bwd<false, false>(dtype, a, stream);
 }
 
-int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+int vitta_top_distill_fwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, int64_t inner_rows,
+                             int64_t outer_stride, float temperature,
                           const int64_t* d_index, const void* d_value, int32_t value_dtype, int32_t list, int32_t tail, float* d_loss,
                           float* d_stats, float* d_q, void* d_workspace, size_t workspace_bytes, uint32_t* d_tickets, void* stream) {
-  if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
+  if (bad_scores(d_x, dtype, rows, classes, row_stride, inner_rows, outer_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || !d_value || !d_loss || bad_stats(d_stats) || !d_q || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
   if (value_dtype < VITTA_SCORES_F32 || value_dtype > VITTA_SCORES_F16) return VITTA_ERR_INVALID_ARG;
   if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   const size_t need = vitta_scores_workspace_bytes(rows, classes, dtype, 0);
   if (workspace_bytes < need || (need && bad_stats(d_workspace))) return VITTA_ERR_WORKSPACE;
   FwdArgs a{};
-  a.x = d_x, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
+  a.x = d_x, a.rows = rows, a.stride = row_stride, a.outer = outer_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
+  a.inner = (uint32_t)(inner_rows < rows ? inner_rows : rows);
   a.stats = d_stats, a.index = d_index, a.value = d_value, a.value_type = value_dtype, a.list = list;
   a.loss = d_loss, a.q = d_q;
   return tail ? launch_fwd<kDistillTail, false, false>(dtype, a, d_workspace, d_tickets, stream) : launch_fwd<kDistill, false, false>(dtype, a, d_workspace, d_tickets, stream);
 }
 
-int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, float temperature,
+int vitta_top_distill_bwd(const void* d_x, int32_t dtype, int64_t rows, int32_t classes, int64_t row_stride, int64_t inner_rows,
+                             int64_t outer_stride, float temperature,
                           const int64_t* d_index, int32_t list, const float* d_stats, const float* d_q, const float* d_g,
                           int64_t g_stride, void* d_dx, void* stream) {
-  if (bad_scores(d_x, dtype, rows, classes, row_stride, temperature)) return VITTA_ERR_INVALID_ARG;
+  if (bad_scores(d_x, dtype, rows, classes, row_stride, inner_rows, outer_stride, temperature)) return VITTA_ERR_INVALID_ARG;
   if (!d_index || bad_stats(d_stats) || !d_q || !d_g || bad_out(d_dx, dtype) || list <= 0 || list > VITTA_SCORES_MAX_LIST) return VITTA_ERR_INVALID_ARG;
   if (too_large(rows, classes)) return VITTA_ERR_UNSUPPORTED;
   BwdArgs a{};
-  a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
+  a.x = d_x, a.dx = d_dx, a.rows = rows, a.stride = row_stride, a.outer = outer_stride, a.classes = classes, a.c = kLog2e / temperature, a.inv_t = 1.f / temperature;
+  a.inner = (uint32_t)(inner_rows < rows ? inner_rows : rows);
   a.stats = d_stats, a.index = d_index, a.list = list, a.q = d_q, a.g = d_g, a.s_g = g_stride;
   return launch_bwd<true, false>(dtype, a, stream);
 }

@@ -183,8 +183,28 @@ def _call(name, index, *args):
         check(status, name)
 
 
+def _row_layout(shape, strides):
+    """(row stride, rows of a group, stride of the groups) of rows whose leading dimensions are at most two groups apart, else None."""
+    if shape[-1] != 1 and strides[-1] != 1:
+        return None
+    groups = []
+    for n, s in zip(shape[:-1], strides[:-1]):
+        if n == 1:
+            continue
+        if groups and groups[-1][1] == n * s:
+            groups[-1] = (groups[-1][0] * n, s)
+        else:
+            groups.append((n, s))
+    if len(groups) > 2:
+        return None
+    if len(groups) < 2:
+        n, s = groups[0] if groups else (1, 0)
+        return s, max(n, 1), 0
+    return groups[1][1], groups[1][0], groups[0][1]
+
+
 def _score_rows(x, name, temperature):
-    """The scores as a matrix whose last stride is 1 (a view; a copy only of what has no such view)."""
+    """(the scores, (rows, classes, row stride, rows of a group, stride of the groups)); copies only what has no such layout."""
     if not x.is_cuda:
         raise _lib.VittaHipError(f"{name} must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
     if x.dtype not in _SCORE_TYPES:
@@ -193,8 +213,15 @@ def _score_rows(x, name, temperature):
         raise ValueError(f"{name} must hold classes in its last dimension (got shape {tuple(x.shape)})")
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"temperature must be a positive finite number (got {temperature})")
-    m = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    return m if m.stride(1) == 1 else m.contiguous()
+    if x.dim() == 2 and x.stride(1) == 1:
+        rows, classes = x.shape
+        return x, (rows, classes, x.stride(0), max(rows, 1), 0)
+    layout = _row_layout(x.shape, x.stride()) if x.numel() else (0, 1, 0)
+    if layout is None:
+        x = x.contiguous()
+        layout = _row_layout(x.shape, x.stride())
+    classes = x.shape[-1]
+    return x, (x.numel() // classes, classes) + layout
 
 
 def _score_side(t, name, like, shape, dtypes):
@@ -242,8 +269,8 @@ def _row_gradient(g):
     return g.contiguous(), 1
 
 
-def _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_index, stats):
-    rows, classes = m.shape
+def _label_logprobs(m, geometry, labels, top, entropy, lse, temperature, ignore_index, stats):
+    rows, classes, lead = geometry[0], geometry[1], m.shape[:-1]
     f32 = torch.float32
     a = b = c = d = e = y = None
     logprob = ent = top_logprob = top_index = None
@@ -264,8 +291,8 @@ def _label_logprobs(m, lead, labels, top, entropy, lse, temperature, ignore_inde
     if rows:
         dtype = _SCORE_TYPES[m.dtype]
         ws, n, tickets = _score_workspace(m, rows, classes, dtype, top)
-        _call("vitta_label_logprobs_fwd", m.get_device(), m.data_ptr(), dtype, rows, classes, m.stride(0), temperature, y, ignore_index, top,
-              a, b, c, d, e, None if stats is None else stats.data_ptr(), None if ws is None else ws.data_ptr(), n, tickets)
+        _call("vitta_label_logprobs_fwd", m.get_device(), m.data_ptr(), dtype, *geometry, temperature, y, ignore_index, top, a, b, c, d, e,
+              None if stats is None else stats.data_ptr(), None if ws is None else ws.data_ptr(), n, tickets)
     return logprob, ent, lse, top_logprob, top_index
 
 
@@ -274,10 +301,10 @@ class _LabelLogprobs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, m, how):
-        stats = m.new_empty((m.shape[0], 4), dtype=torch.float32)
+        stats = m.new_empty((how[0][0], 4), dtype=torch.float32)
         out = _label_logprobs(m, *how, stats)
         ctx.save_for_backward(m, how[1], out[4], stats)
-        ctx.how = how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
+        ctx.how = how[0], how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
         if how[2]:
             ctx.mark_non_differentiable(out[4])
         ctx.set_materialize_grads(False)
@@ -290,10 +317,9 @@ class _LabelLogprobs(torch.autograd.Function):
 
 def _label_logprobs_grad(ctx, *upstream):
     m, labels, top_index, stats = ctx.saved_tensors
-    top, temperature, ignore_index, asked = ctx.how
-    rows, classes = m.shape
-    dx = m.new_empty((rows, classes))
-    if rows:
+    geometry, top, temperature, ignore_index, asked = ctx.how
+    dx = m.new_empty(m.shape)
+    if geometry[0]:
         at, stride, index, label = [None] * 4, [0] * 3, None, None
         keep = []  # (dense copies live until the launch is issued)
         for i, g in zip(asked, upstream):
@@ -307,8 +333,8 @@ def _label_logprobs_grad(ctx, *upstream):
                     label = labels.data_ptr()
             keep.append(g)
             at[i] = g.data_ptr()
-        _call("vitta_label_logprobs_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), temperature, label,
-              ignore_index, top, index, stats.data_ptr(), at[0], stride[0], at[1], stride[1], at[2], stride[2], at[3], dx.data_ptr())
+        _call("vitta_label_logprobs_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], *geometry, temperature, label, ignore_index,
+              top, index, stats.data_ptr(), at[0], stride[0], at[1], stride[1], at[2], stride[2], at[3], dx.data_ptr())
     return dx, None
 
 
@@ -318,7 +344,8 @@ _label_logprobs_again = once_differentiable(_label_logprobs_grad)  # (under crea
 def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, temperature=1.0, ignore_index=-100):
     """Log probability of given labels, entropy and best alternatives of rows of class scores, read once.
 
-    logits (..., V) float32 / bfloat16 / float16 (rows may be cut from a wider matrix; V at most 2 ** 24); labels (...) int64 or int32, or
+    logits (..., V) float32 / bfloat16 / float16 (rows may be cut from a wider matrix or from
+    sequences, logits[:, :-1]; V at most 2 ** 24); labels (...) int64 or int32, or
     None.
     Returns a LabelLogprobs of float32 tensors shaped (...): with z = logits / temperature,
       logprob       z[label] - lse; 0 where label == ignore_index; NaN where the label is no class (None without labels)
@@ -328,15 +355,14 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
                     log probability -inf where fewer classes have a score above -inf.
     A row of -inf only has log probabilities -inf, entropy 0 and gradient 0; a row with NaN or +inf answers NaN and -1.
     Differentiable once in logits through logprob, entropy, lse and top_logprob; the gradient has the logits' type."""
-    m = _score_rows(logits, "logits", temperature)
-    if not 0 <= top <= min(_lib.SCORES_MAX_TOP, m.shape[1]):
-        raise ValueError(f"top must be between 0 and min({_lib.SCORES_MAX_TOP}, classes = {m.shape[1]}) (got {top})")
+    m, geometry = _score_rows(logits, "logits", temperature)
+    if not 0 <= top <= min(_lib.SCORES_MAX_TOP, geometry[1]):
+        raise ValueError(f"top must be between 0 and min({_lib.SCORES_MAX_TOP}, classes = {geometry[1]}) (got {top})")
     if labels is None and not (top or entropy or lse):
         raise ValueError("nothing is asked: give labels, top, entropy or lse")
-    lead = logits.shape[:-1]
     if labels is not None:
-        labels = _score_side(labels, "labels", logits, lead, (torch.int64, torch.int32))
-    how = lead, labels, int(top), entropy, lse, float(temperature), int(ignore_index)
+        labels = _score_side(labels, "labels", logits, logits.shape[:-1], (torch.int64, torch.int32))
+    how = geometry, labels, int(top), entropy, lse, float(temperature), int(ignore_index)
     if not (m.requires_grad and torch.is_grad_enabled()):
         return LabelLogprobs(*_label_logprobs(m, *how, None))
     out = iter(_LabelLogprobs.apply(m, how))
@@ -344,19 +370,18 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
                          next(out) if top else None, next(out) if top else None)
 
 
-def _top_distill(m, lead, index, value, temperature, tail):
+def _top_distill(m, geometry, index, value, temperature, tail):
     """(loss, the row statistics (rows, 4) and the teacher's probabilities (rows, k) in one buffer)"""
-    rows, classes = m.shape
+    rows, classes = geometry[:2]
     k = index.shape[-1]
-    loss = m.new_empty(lead, dtype=torch.float32)
+    loss = m.new_empty(m.shape[:-1], dtype=torch.float32)
     side = m.new_empty(rows * (4 + k), dtype=torch.float32)
     if rows:
         dtype = _SCORE_TYPES[m.dtype]
         ws, n, tickets = _score_workspace(m, rows, classes, dtype, 0)
         stats = side.data_ptr()
-        _call("vitta_top_distill_fwd", m.get_device(), m.data_ptr(), dtype, rows, classes, m.stride(0), temperature, index.data_ptr(),
-              value.data_ptr(), _SCORE_TYPES[value.dtype], k, tail, loss.data_ptr(), stats, stats + 16 * rows,
-              None if ws is None else ws.data_ptr(), n, tickets)
+        _call("vitta_top_distill_fwd", m.get_device(), m.data_ptr(), dtype, *geometry, temperature, index.data_ptr(), value.data_ptr(),
+              _SCORE_TYPES[value.dtype], k, tail, loss.data_ptr(), stats, stats + 16 * rows, None if ws is None else ws.data_ptr(), n, tickets)
     return loss, side
 
 
@@ -367,7 +392,7 @@ class _TopDistill(torch.autograd.Function):
     def forward(ctx, m, how):
         loss, side = _top_distill(m, *how)
         ctx.save_for_backward(m, how[1], side)
-        ctx.temperature = how[3]
+        ctx.how = how[0], how[3]
         return loss
 
     @staticmethod
@@ -377,13 +402,13 @@ class _TopDistill(torch.autograd.Function):
 
 def _top_distill_grad(ctx, g):
     m, index, side = ctx.saved_tensors
-    rows, classes = m.shape
-    dx = m.new_empty((rows, classes))
-    if rows:
+    geometry, temperature = ctx.how
+    dx = m.new_empty(m.shape)
+    if geometry[0]:
         g, stride = _row_gradient(g)
         stats = side.data_ptr()
-        _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], rows, classes, m.stride(0), ctx.temperature,
-              index.data_ptr(), index.shape[-1], stats, stats + 16 * rows, g.data_ptr(), stride, dx.data_ptr())
+        _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], *geometry, temperature, index.data_ptr(),
+              index.shape[-1], stats, stats + 16 * geometry[0], g.data_ptr(), stride, dx.data_ptr())
     return dx, None
 
 
@@ -401,16 +426,15 @@ def top_distill(student_logits, teacher_index, teacher_value, *, temperature=1.0
                   student gives the classes outside the list (left out where that is nothing).
     A class listed twice counts with the sum of its probabilities.  No factor temperature ** 2 is applied.  Differentiable once in
     student_logits; the gradient has their type."""
-    m = _score_rows(student_logits, "student_logits", temperature)
+    m, geometry = _score_rows(student_logits, "student_logits", temperature)
     if teacher_index.dim() == 0 or not 1 <= teacher_index.shape[-1] <= _lib.SCORES_MAX_LIST:
         raise ValueError(f"teacher_index must hold 1 to {_lib.SCORES_MAX_LIST} classes per row (got shape {tuple(teacher_index.shape)})")
     if teacher_value.requires_grad:
         raise ValueError("teacher_value gets no gradient: detach it")
-    lead = student_logits.shape[:-1]
-    shape = lead + teacher_index.shape[-1:]
+    shape = student_logits.shape[:-1] + teacher_index.shape[-1:]
     index = _score_side(teacher_index, "teacher_index", student_logits, shape, (torch.int64, torch.int32))
     value = _score_side(teacher_value, "teacher_value", student_logits, shape, _SCORE_TYPES)
-    how = lead, index, value, float(temperature), bool(tail)
+    how = geometry, index, value, float(temperature), bool(tail)
     if m.requires_grad and torch.is_grad_enabled():
         return _TopDistill.apply(m, how)
     return _top_distill(m, *how)[0]
