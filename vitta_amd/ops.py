@@ -203,16 +203,8 @@ def _row_layout(shape, strides):
     return groups[1][1], groups[1][0], groups[0][1]
 
 
-def _score_rows(x, name, temperature):
+def _rows_of(x):
     """(the scores, (rows, classes, row stride, rows of a group, stride of the groups)); copies only what has no such layout."""
-    if not x.is_cuda:
-        raise _lib.VittaHipError(f"{name} must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
-    if x.dtype not in _SCORE_TYPES:
-        raise _lib.VittaHipError(f"{name} must be float32, bfloat16 or float16 (got {x.dtype})")
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"{name} must hold classes in its last dimension (got shape {tuple(x.shape)})")
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"temperature must be a positive finite number (got {temperature})")
     if x.dim() == 2 and x.stride(1) == 1:
         rows, classes = x.shape
         return x, (rows, classes, x.stride(0), max(rows, 1), 0)
@@ -222,6 +214,27 @@ def _score_rows(x, name, temperature):
         layout = _row_layout(x.shape, x.stride())
     classes = x.shape[-1]
     return x, (x.numel() // classes, classes) + layout
+
+
+def _score_rows(x, name, temperature):
+    """_rows_of what the operators take for scores"""
+    if not x.is_cuda:
+        raise _lib.VittaHipError(f"{name} must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
+    if x.dtype not in _SCORE_TYPES:
+        raise _lib.VittaHipError(f"{name} must be float32, bfloat16 or float16 (got {x.dtype})")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{name} must hold classes in its last dimension (got shape {tuple(x.shape)})")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature must be a positive finite number (got {temperature})")
+    return _rows_of(x)
+
+
+def _saved(t, device, shape, dtype, name):
+    """A tensor as the forward saved it.  Saved-tensor hooks (torch.autograd.graph.save_on_cpu for one) may give it back in another layout, so
+    a backward takes strides and addresses from what it is given, never from the forward; another type, shape or device is an error."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise _lib.VittaHipError(f"the saved {name} came back as {t.dtype} {tuple(t.shape)} on {t.device} (saved: {dtype} {tuple(shape)})")
+    return t
 
 
 def _score_side(t, name, like, shape, dtypes):
@@ -304,7 +317,8 @@ class _LabelLogprobs(torch.autograd.Function):
         stats = m.new_empty((how[0][0], 4), dtype=torch.float32)
         out = _label_logprobs(m, *how, stats)
         ctx.save_for_backward(m, how[1], out[4], stats)
-        ctx.how = how[0], how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
+        ctx.scores = m.shape, m.dtype, m.device
+        ctx.how = how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
         if how[2]:
             ctx.mark_non_differentiable(out[4])
         ctx.set_materialize_grads(False)
@@ -317,23 +331,29 @@ class _LabelLogprobs(torch.autograd.Function):
 
 def _label_logprobs_grad(ctx, *upstream):
     m, labels, top_index, stats = ctx.saved_tensors
-    geometry, top, temperature, ignore_index, asked = ctx.how
-    dx = m.new_empty(m.shape)
-    if geometry[0]:
+    shape, dtype, device = ctx.scores
+    top, temperature, ignore_index, asked = ctx.how
+    m, geometry = _rows_of(_saved(m, device, shape, dtype, "scores"))
+    rows, lead = geometry[0], shape[:-1]
+    dx = m.new_empty(shape)
+    if rows:
+        stats = _saved(stats, device, (rows, 4), torch.float32, "statistics").contiguous()
         at, stride, index, label = [None] * 4, [0] * 3, None, None
         keep = []  # (dense copies live until the launch is issued)
         for i, g in zip(asked, upstream):
             if g is None:
                 continue
             if i == 3:
+                top_index = _saved(top_index, device, lead + (top,), torch.int64, "alternatives").contiguous()
                 g, index = g.contiguous(), top_index.data_ptr()
             else:
                 g, stride[i] = _row_gradient(g)
                 if i == 0:
+                    labels = _saved(labels, device, lead, torch.int64, "labels").contiguous()
                     label = labels.data_ptr()
             keep.append(g)
             at[i] = g.data_ptr()
-        _call("vitta_label_logprobs_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], *geometry, temperature, label, ignore_index,
+        _call("vitta_label_logprobs_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, label, ignore_index,
               top, index, stats.data_ptr(), at[0], stride[0], at[1], stride[1], at[2], stride[2], at[3], dx.data_ptr())
     return dx, None
 
@@ -392,7 +412,8 @@ class _TopDistill(torch.autograd.Function):
     def forward(ctx, m, how):
         loss, side = _top_distill(m, *how)
         ctx.save_for_backward(m, how[1], side)
-        ctx.how = how[0], how[3]
+        ctx.scores = m.shape, m.dtype, m.device
+        ctx.how = how[1].shape, how[3]
         return loss
 
     @staticmethod
@@ -402,13 +423,18 @@ class _TopDistill(torch.autograd.Function):
 
 def _top_distill_grad(ctx, g):
     m, index, side = ctx.saved_tensors
-    geometry, temperature = ctx.how
-    dx = m.new_empty(m.shape)
-    if geometry[0]:
+    shape, dtype, device = ctx.scores
+    listed, temperature = ctx.how
+    m, geometry = _rows_of(_saved(m, device, shape, dtype, "scores"))
+    rows, k = geometry[0], listed[-1]
+    dx = m.new_empty(shape)
+    if rows:
         g, stride = _row_gradient(g)
+        index = _saved(index, device, listed, torch.int64, "list").contiguous()
+        side = _saved(side, device, (rows * (4 + k),), torch.float32, "statistics").contiguous()
         stats = side.data_ptr()
-        _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[m.dtype], *geometry, temperature, index.data_ptr(),
-              index.shape[-1], stats, stats + 16 * geometry[0], g.data_ptr(), stride, dx.data_ptr())
+        _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, index.data_ptr(), k, stats,
+              stats + 16 * rows, g.data_ptr(), stride, dx.data_ptr())
     return dx, None
 
 
