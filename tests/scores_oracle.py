@@ -114,15 +114,17 @@ def distill(x, index, value, temperature=1.0, tail=False):
         p = torch.exp(lp[r])
         spread = torch.where(p > 0, (x[r].double() - x[r].double().max()).abs() / temperature, torch.zeros_like(p))
         rel = U * (depth(classes) + len(entries) + 60)
-        by = {}
+        by, size = {}, {}  # a class listed more than once is one class with the sum of its probabilities
         for (i, v), qk in zip(entries, q):
+            by[i] = by.get(i, 0.0) + qk
+            size[i] = max(size.get(i, 0.0), abs(v) if qk > 0 else 0.0)
+        for i, qk in by.items():
             if qk > 0:
-                log_q = v if tail else math.log(qk)
-                far = abs(log_q) + abs(float(lp[r, i])) + abs(v) / scale + float(spread[i])
+                log_q = math.log(qk)
+                far = abs(log_q) + abs(float(lp[r, i])) + size[i] / scale + float(spread[i])
                 loss[r] += qk * (log_q - float(lp[r, i]))
                 # (q itself is off by (8 |v| + len) u, its logarithm by that much, the student's by rel + 8 u spread)
                 e_loss[r] += qk * (rel * (1 + far) + 8 * U * far * (1 + far))
-            by[i] = by.get(i, 0.0) + qk
         every = sum(q)
         e_every = every * U * (len(entries) + 16 + 8 * max(abs(v) for _, v in entries) / scale)
         inside = outside = every

@@ -337,19 +337,19 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
     vm = fmaxf(vm, val[i]);
   }
   some = __ballot(some) != 0;
+  uint32_t again = 0;  // bit i: at[i] stands earlier in the list already
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int n = min(64, K - i * 64);
+    for (int l = 0; l < n; ++l) {
+      const int32_t j = __builtin_amdgcn_readlane(at[i], l);
+#pragma unroll
+      for (int o = i; o < R; ++o)
+        if (o * 64 < K && at[o] == j && (o > i || lane > l)) again |= 1u << o;
+    }
+  }
   float m = v.m, s = v.s, rest = 0.f;
   if (TAIL) {  // the listed classes' own sum, each once
-    uint32_t again = 0;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int n = min(64, K - i * 64);
-      for (int l = 0; l < n; ++l) {
-        const int32_t j = __builtin_amdgcn_readlane(at[i], l);
-#pragma unroll
-        for (int o = 0; o < R; ++o)
-          if (at[o] == j && o * 64 + lane > i * 64 + l) again |= 1u << o;
-      }
-    }
 #pragma unroll
     for (int i = 0; i < R; ++i) m = fmaxf(m, z[i]);
     m = all_max(m, lane);
@@ -370,17 +370,36 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
   }
   sum = all_sum(sum, lane);
   const float inv = TAIL ? 1.f : 1.f / sum, ql = TAIL ? 0.f : kLn2 * log2_fast(sum);
+  float log_q[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    q[i] *= at[i] >= 0 ? inv : 0.f;
+    log_q[i] = TAIL ? val[i] : below(val[i], ref, A.inv_t) - ql;
+  }
+  bool repeats = false;
+#pragma unroll
+  for (int i = 0; i < R; ++i) repeats |= at[i] >= 0 && (again >> i & 1);
+  if (__ballot(repeats) != 0) {  // a class listed more than once is one class with the sum of its probabilities
+    float all[R] = {};
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int n = min(64, K - i * 64);
+      for (int l = 0; l < n; ++l) {
+        const int32_t j = __builtin_amdgcn_readlane(at[i], l);
+        const float more = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q[i]), l));
+#pragma unroll
+        for (int o = 0; o < R; ++o) all[o] += at[o] == j ? more : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (all[i] != q[i]) log_q[i] = kLn2 * log2_fast(all[i]);
+  }
   float loss = 0.f;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int k = i * 64 + lane;
-    if (at[i] >= 0) {
-      q[i] *= inv;
-      if (q[i] != 0.f) {
-        const float log_q = TAIL ? val[i] : below(val[i], ref, A.inv_t) - ql;
-        loss += q[i] * (log_q - (s == 0.f ? -INFINITY : below(z[i], m, A.inv_t) - kLn2 * l2));
-      }
-    }
+    if (at[i] >= 0 && q[i] != 0.f) loss += q[i] * (log_q[i] - (s == 0.f ? -INFINITY : below(z[i], m, A.inv_t) - kLn2 * l2));
     if (k < K) A.q[row * K + k] = q[i];
   }
   loss = all_sum(loss, lane);
