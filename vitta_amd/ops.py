@@ -204,16 +204,17 @@ def _row_layout(shape, strides):
 
 
 def _rows_of(x):
-    """(the scores, (rows, classes, row stride, rows of a group, stride of the groups)); copies only what has no such layout."""
-    if x.dim() == 2 and x.stride(1) == 1:
-        rows, classes = x.shape
-        return x, (rows, classes, x.stride(0), max(rows, 1), 0)
-    layout = _row_layout(x.shape, x.stride()) if x.numel() else (0, 1, 0)
+    """(the scores, (shape, type, device, strides, (rows, classes, row stride, rows of a group, stride of the groups), leading shape)); copies
+    only what has no such layout."""
+    shape, stride = x.shape, x.stride()
+    if len(shape) == 2 and stride[1] == 1:
+        return x, (shape, x.dtype, x.device, stride, (shape[0], shape[1], stride[0], shape[0] or 1, 0), shape[:1])
+    layout = _row_layout(shape, stride) if x.numel() else (0, 1, 0)
     if layout is None:
         x = x.contiguous()
-        layout = _row_layout(x.shape, x.stride())
-    classes = x.shape[-1]
-    return x, (x.numel() // classes, classes) + layout
+        stride = x.stride()
+        layout = _row_layout(shape, stride)
+    return x, (shape, x.dtype, x.device, stride, (x.numel() // shape[-1], shape[-1]) + layout, shape[:-1])
 
 
 def _score_rows(x, name, temperature):
@@ -229,18 +230,26 @@ def _score_rows(x, name, temperature):
     return _rows_of(x)
 
 
-def _saved(t, device, shape, dtype, name):
-    """A tensor as the forward saved it.  Saved-tensor hooks (torch.autograd.graph.save_on_cpu for one) may give it back in another layout, so
-    a backward takes strides and addresses from what it is given, never from the forward; another type, shape or device is an error."""
-    if t.shape != shape or t.dtype != dtype or t.device != device:
-        raise _lib.VittaHipError(f"the saved {name} came back as {t.dtype} {tuple(t.shape)} on {t.device} (saved: {dtype} {tuple(shape)})")
-    return t
+def _saved(t, shape, dtype, device, name):
+    """A tensor as the forward saved it, dense.  Saved-tensor hooks (torch.autograd.graph.save_on_cpu for one) may give it back in another
+    layout, so a backward takes strides and addresses from what it is given, never from the forward; another type, shape or device is an error."""
+    if t.shape == shape and t.dtype is dtype and t.device == device:
+        return t.contiguous()
+    raise _lib.VittaHipError(f"the saved {name} came back as {t.dtype} {tuple(t.shape)} on {t.device} (saved: {dtype} {tuple(shape)} on {device})")
 
 
-def _score_side(t, name, like, shape, dtypes):
+def _saved_rows(m, shape, dtype, device):
+    """(the saved scores, their geometry) where hooks have changed their layout"""
+    if m.shape != shape or m.dtype is not dtype or m.device != device:
+        _saved(m, shape, dtype, device, "scores")
+    m, scores = _rows_of(m)
+    return m, scores[4]
+
+
+def _score_side(t, name, device, shape, dtypes):
     """A companion of the scores (labels, a teacher's list): on their device, of the given shape and one of the types, dense."""
-    if t.device != like.device:
-        raise _lib.VittaHipError(f"{name} must live on {like.device} like the scores (got {t.device})")
+    if t.device != device:
+        raise _lib.VittaHipError(f"{name} must live on {device} like the scores (got {t.device})")
     if t.dtype not in dtypes:
         raise _lib.VittaHipError(f"{name} must be one of {[str(d) for d in dtypes]} (got {t.dtype})")
     if t.shape != shape:
@@ -282,8 +291,9 @@ def _row_gradient(g):
     return g.contiguous(), 1
 
 
-def _label_logprobs(m, geometry, labels, top, entropy, lse, temperature, ignore_index, stats):
-    rows, classes, lead = geometry[0], geometry[1], m.shape[:-1]
+def _label_logprobs(m, scores, labels, top, entropy, lse, temperature, ignore_index, stats):
+    _, dtype, _, _, geometry, lead = scores
+    rows, classes = geometry[:2]
     f32 = torch.float32
     a = b = c = d = e = y = None
     logprob = ent = top_logprob = top_index = None
@@ -302,7 +312,7 @@ def _label_logprobs(m, geometry, labels, top, entropy, lse, temperature, ignore_
         top_logprob, top_index = m.new_empty((*lead, top), dtype=f32), m.new_empty((*lead, top), dtype=torch.int64)
         d, e = top_logprob.data_ptr(), top_index.data_ptr()
     if rows:
-        dtype = _SCORE_TYPES[m.dtype]
+        dtype = _SCORE_TYPES[dtype]
         ws, n, tickets = _score_workspace(m, rows, classes, dtype, top)
         _call("vitta_label_logprobs_fwd", m.get_device(), m.data_ptr(), dtype, *geometry, temperature, y, ignore_index, top, a, b, c, d, e,
               None if stats is None else stats.data_ptr(), None if ws is None else ws.data_ptr(), n, tickets)
@@ -314,11 +324,11 @@ class _LabelLogprobs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, m, how):
-        stats = m.new_empty((how[0][0], 4), dtype=torch.float32)
+        stats = m.new_empty((how[0][4][0], 4), dtype=torch.float32)
         out = _label_logprobs(m, *how, stats)
-        ctx.save_for_backward(m, how[1], out[4], stats)
-        ctx.scores = m.shape, m.dtype, m.device
-        ctx.how = how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
+        ctx.save_for_backward(m, how[1], out[4])
+        # (the statistics, 16 bytes a row that only the backward knows, stay on the node, where no hook changes their layout)
+        ctx.how = how[0], stats, how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
         if how[2]:
             ctx.mark_non_differentiable(out[4])
         ctx.set_materialize_grads(False)
@@ -330,26 +340,25 @@ class _LabelLogprobs(torch.autograd.Function):
 
 
 def _label_logprobs_grad(ctx, *upstream):
-    m, labels, top_index, stats = ctx.saved_tensors
-    shape, dtype, device = ctx.scores
-    top, temperature, ignore_index, asked = ctx.how
-    m, geometry = _rows_of(_saved(m, device, shape, dtype, "scores"))
-    rows, lead = geometry[0], shape[:-1]
+    m, labels, top_index = ctx.saved_tensors
+    scores, stats, top, temperature, ignore_index, asked = ctx.how
+    shape, dtype, device, strides, geometry, lead = scores
+    if not (m.stride() == strides and m.shape == shape and m.dtype is dtype and m.device == device):
+        m, geometry = _saved_rows(m, shape, dtype, device)
     dx = m.new_empty(shape)
-    if rows:
-        stats = _saved(stats, device, (rows, 4), torch.float32, "statistics").contiguous()
+    if geometry[0]:
         at, stride, index, label = [None] * 4, [0] * 3, None, None
         keep = []  # (dense copies live until the launch is issued)
         for i, g in zip(asked, upstream):
             if g is None:
                 continue
             if i == 3:
-                top_index = _saved(top_index, device, lead + (top,), torch.int64, "alternatives").contiguous()
+                top_index = _saved(top_index, lead + (top,), torch.int64, device, "alternatives")
                 g, index = g.contiguous(), top_index.data_ptr()
             else:
                 g, stride[i] = _row_gradient(g)
                 if i == 0:
-                    labels = _saved(labels, device, lead, torch.int64, "labels").contiguous()
+                    labels = _saved(labels, lead, torch.int64, device, "labels")
                     label = labels.data_ptr()
             keep.append(g)
             at[i] = g.data_ptr()
@@ -375,14 +384,14 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
                     log probability -inf where fewer classes have a score above -inf.
     A row of -inf only has log probabilities -inf, entropy 0 and gradient 0; a row with NaN or +inf answers NaN and -1.
     Differentiable once in logits through logprob, entropy, lse and top_logprob; the gradient has the logits' type."""
-    m, geometry = _score_rows(logits, "logits", temperature)
-    if not 0 <= top <= min(_lib.SCORES_MAX_TOP, geometry[1]):
-        raise ValueError(f"top must be between 0 and min({_lib.SCORES_MAX_TOP}, classes = {geometry[1]}) (got {top})")
+    m, scores = _score_rows(logits, "logits", temperature)
+    if not 0 <= top <= min(_lib.SCORES_MAX_TOP, scores[4][1]):
+        raise ValueError(f"top must be between 0 and min({_lib.SCORES_MAX_TOP}, classes = {scores[4][1]}) (got {top})")
     if labels is None and not (top or entropy or lse):
         raise ValueError("nothing is asked: give labels, top, entropy or lse")
     if labels is not None:
-        labels = _score_side(labels, "labels", logits, logits.shape[:-1], (torch.int64, torch.int32))
-    how = geometry, labels, int(top), entropy, lse, float(temperature), int(ignore_index)
+        labels = _score_side(labels, "labels", scores[2], scores[5], (torch.int64, torch.int32))
+    how = scores, labels, int(top), entropy, lse, float(temperature), int(ignore_index)
     if not (m.requires_grad and torch.is_grad_enabled()):
         return LabelLogprobs(*_label_logprobs(m, *how, None))
     out = iter(_LabelLogprobs.apply(m, how))
@@ -390,14 +399,15 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
                          next(out) if top else None, next(out) if top else None)
 
 
-def _top_distill(m, geometry, index, value, temperature, tail):
+def _top_distill(m, scores, index, value, temperature, tail):
     """(loss, the row statistics (rows, 4) and the teacher's probabilities (rows, k) in one buffer)"""
+    _, dtype, _, _, geometry, lead = scores
     rows, classes = geometry[:2]
     k = index.shape[-1]
-    loss = m.new_empty(m.shape[:-1], dtype=torch.float32)
+    loss = m.new_empty(lead, dtype=torch.float32)
     side = m.new_empty(rows * (4 + k), dtype=torch.float32)
     if rows:
-        dtype = _SCORE_TYPES[m.dtype]
+        dtype = _SCORE_TYPES[dtype]
         ws, n, tickets = _score_workspace(m, rows, classes, dtype, 0)
         stats = side.data_ptr()
         _call("vitta_top_distill_fwd", m.get_device(), m.data_ptr(), dtype, *geometry, temperature, index.data_ptr(), value.data_ptr(),
@@ -411,9 +421,8 @@ class _TopDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, m, how):
         loss, side = _top_distill(m, *how)
-        ctx.save_for_backward(m, how[1], side)
-        ctx.scores = m.shape, m.dtype, m.device
-        ctx.how = how[1].shape, how[3]
+        ctx.save_for_backward(m, how[1])
+        ctx.how = how[0], side, how[1].shape, how[3]  # (the statistics as above)
         return loss
 
     @staticmethod
@@ -422,19 +431,18 @@ class _TopDistill(torch.autograd.Function):
 
 
 def _top_distill_grad(ctx, g):
-    m, index, side = ctx.saved_tensors
-    shape, dtype, device = ctx.scores
-    listed, temperature = ctx.how
-    m, geometry = _rows_of(_saved(m, device, shape, dtype, "scores"))
-    rows, k = geometry[0], listed[-1]
+    m, index = ctx.saved_tensors
+    scores, side, listed, temperature = ctx.how
+    shape, dtype, device, strides, geometry, _ = scores
+    if not (m.stride() == strides and m.shape == shape and m.dtype is dtype and m.device == device):
+        m, geometry = _saved_rows(m, shape, dtype, device)
     dx = m.new_empty(shape)
-    if rows:
+    if geometry[0]:
         g, stride = _row_gradient(g)
-        index = _saved(index, device, listed, torch.int64, "list").contiguous()
-        side = _saved(side, device, (rows * (4 + k),), torch.float32, "statistics").contiguous()
+        index = _saved(index, listed, torch.int64, device, "list")
         stats = side.data_ptr()
-        _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, index.data_ptr(), k, stats,
-              stats + 16 * rows, g.data_ptr(), stride, dx.data_ptr())
+        _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, index.data_ptr(), listed[-1],
+              stats, stats + 16 * geometry[0], g.data_ptr(), stride, dx.data_ptr())
     return dx, None
 
 
@@ -452,15 +460,15 @@ def top_distill(student_logits, teacher_index, teacher_value, *, temperature=1.0
                   student gives the classes outside the list (left out where that is nothing).
     A class listed twice counts with the sum of its probabilities.  No factor temperature ** 2 is applied.  Differentiable once in
     student_logits; the gradient has their type."""
-    m, geometry = _score_rows(student_logits, "student_logits", temperature)
+    m, scores = _score_rows(student_logits, "student_logits", temperature)
     if teacher_index.dim() == 0 or not 1 <= teacher_index.shape[-1] <= _lib.SCORES_MAX_LIST:
         raise ValueError(f"teacher_index must hold 1 to {_lib.SCORES_MAX_LIST} classes per row (got shape {tuple(teacher_index.shape)})")
     if teacher_value.requires_grad:
         raise ValueError("teacher_value gets no gradient: detach it")
-    shape = student_logits.shape[:-1] + teacher_index.shape[-1:]
-    index = _score_side(teacher_index, "teacher_index", student_logits, shape, (torch.int64, torch.int32))
-    value = _score_side(teacher_value, "teacher_value", student_logits, shape, _SCORE_TYPES)
-    how = geometry, index, value, float(temperature), bool(tail)
+    shape = scores[5] + teacher_index.shape[-1:]
+    index = _score_side(teacher_index, "teacher_index", scores[2], shape, (torch.int64, torch.int32))
+    value = _score_side(teacher_value, "teacher_value", scores[2], shape, _SCORE_TYPES)
+    how = scores, index, value, float(temperature), bool(tail)
     if m.requires_grad and torch.is_grad_enabled():
         return _TopDistill.apply(m, how)
     return _top_distill(m, *how)[0]
