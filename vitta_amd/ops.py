@@ -10,6 +10,7 @@ from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -166,6 +167,7 @@ class LabelLogprobs(NamedTuple):
 # These calls are short (a batch of class scores is a few microseconds of GPU time), so their host side is kept lean: plain integers to
 # ctypes, the raw stream, a device switch only where the tensors are not on the current device.
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_tracing, _modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
 _entry_points = {}
 
 
@@ -219,6 +221,9 @@ def _rows_of(x):
 
 def _score_rows(x, name, temperature):
     """_rows_of what the operators take for scores"""
+    # a tracer records what torch does, and a launch is not among it: the program would answer with uninitialised memory
+    if _tracing() is not None or _modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise _lib.VittaHipError("the score operators cannot be traced: a launch leaves no record")
     if not x.is_cuda:
         raise _lib.VittaHipError(f"{name} must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
     if x.dtype not in _SCORE_TYPES:
@@ -244,6 +249,12 @@ def _saved_rows(m, shape, dtype, device):
         _saved(m, shape, dtype, device, "scores")
     m, scores = _rows_of(m)
     return m, scores[4]
+
+
+def _recorded(m):
+    """Whether a call goes through autograd: for a gradient, and in a forward-mode level, where Function.apply refuses a tangent (there is no
+    rule for one) that the plain call would drop."""
+    return m.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0
 
 
 def _score_side(t, name, device, shape, dtypes):
@@ -383,7 +394,8 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
       top_logprob, top_index (..., top): the `top` (at most 64) best classes in falling order, ties to the lowest index; index -1 and
                     log probability -inf where fewer classes have a score above -inf.
     A row of -inf only has log probabilities -inf, entropy 0 and gradient 0; a row with NaN or +inf answers NaN and -1.
-    Differentiable once in logits through logprob, entropy, lse and top_logprob; the gradient has the logits' type."""
+    Differentiable once in logits through logprob, entropy, lse and top_logprob; the gradient has the logits' type.  Forward-mode tangents
+    and tracers (torch.jit.trace, make_fx) are refused."""
     m, scores = _score_rows(logits, "logits", temperature)
     if not 0 <= top <= min(_lib.SCORES_MAX_TOP, scores[4][1]):
         raise ValueError(f"top must be between 0 and min({_lib.SCORES_MAX_TOP}, classes = {scores[4][1]}) (got {top})")
@@ -392,7 +404,7 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
     if labels is not None:
         labels = _score_side(labels, "labels", scores[2], scores[5], (torch.int64, torch.int32))
     how = scores, labels, int(top), entropy, lse, float(temperature), int(ignore_index)
-    if not (m.requires_grad and torch.is_grad_enabled()):
+    if not _recorded(m):
         return LabelLogprobs(*_label_logprobs(m, *how, None))
     out = iter(_LabelLogprobs.apply(m, how))
     return LabelLogprobs(next(out) if labels is not None else None, next(out) if entropy else None, next(out) if lse else None,
@@ -459,17 +471,17 @@ def top_distill(student_logits, teacher_index, teacher_value, *, temperature=1.0
       tail=True   teacher_value are log probabilities (at the same temperature); what they leave of 1 is one more class against what the
                   student gives the classes outside the list (left out where that is nothing).
     A class listed twice counts with the sum of its probabilities.  No factor temperature ** 2 is applied.  Differentiable once in
-    student_logits; the gradient has their type."""
+    student_logits; the gradient has their type.  Forward-mode tangents and tracers are refused, as by `label_logprobs`."""
     m, scores = _score_rows(student_logits, "student_logits", temperature)
     if teacher_index.dim() == 0 or not 1 <= teacher_index.shape[-1] <= _lib.SCORES_MAX_LIST:
         raise ValueError(f"teacher_index must hold 1 to {_lib.SCORES_MAX_LIST} classes per row (got shape {tuple(teacher_index.shape)})")
-    if teacher_value.requires_grad:
+    if teacher_value.requires_grad or forward_ad._current_level >= 0 and forward_ad.unpack_dual(teacher_value).tangent is not None:
         raise ValueError("teacher_value gets no gradient: detach it")
     shape = scores[5] + teacher_index.shape[-1:]
     index = _score_side(teacher_index, "teacher_index", scores[2], shape, (torch.int64, torch.int32))
     value = _score_side(teacher_value, "teacher_value", scores[2], shape, _SCORE_TYPES)
     how = scores, index, value, float(temperature), bool(tail)
-    if m.requires_grad and torch.is_grad_enabled():
+    if _recorded(m):
         return _TopDistill.apply(m, how)
     return _top_distill(m, *how)[0]
 
