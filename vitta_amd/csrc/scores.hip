@@ -140,6 +140,14 @@ template <class Op> __device__ __forceinline__ float wave_all(float v, int lane,
 }
 __device__ __forceinline__ float all_max(float v, int lane) { return wave_all(v, lane, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float all_sum(float v, int lane) { return wave_all(v, lane, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ double all_sum(double v, int lane) {
+  v += __longlong_as_double((long long)lane_xor<1>((uint64_t)__double_as_longlong(v), lane));
+  v += __longlong_as_double((long long)lane_xor<2>((uint64_t)__double_as_longlong(v), lane));
+  v += __longlong_as_double((long long)lane_xor<4>((uint64_t)__double_as_longlong(v), lane));
+  v += __longlong_as_double((long long)lane_xor<8>((uint64_t)__double_as_longlong(v), lane));
+  v += __longlong_as_double((long long)lane_xor<16>((uint64_t)__double_as_longlong(v), lane));
+  return v + __longlong_as_double((long long)lane_xor<32>((uint64_t)__double_as_longlong(v), lane));
+}
 
 // ---- running sums ----------------------------------------------------------------------------------------------------------------
 // (max, sum of 2^a, sum of a 2^a); a is clamped where its power is 0 anyway, so that 0 * -inf never forms (a NaN reaches s unclamped)
@@ -361,14 +369,29 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
     s = rest + all_sum(in, lane);
   }
   const float l2 = log2_fast(s);
-  const float ref = TAIL ? 0.f : all_max(vm, lane), cv = TAIL ? kLog2e : A.c;
-  float q[R], sum = 0.f;
+  const float ref = TAIL ? 0.f : all_max(vm, lane);
+  float q[R], sum = 0.f, q_rest = 0.f;
+  if (TAIL) {  // in 64 bits, once a row: 32 bits of 1 - sum are all lost where a confident teacher leaves 1e-7
+    double in = 0.;
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    q[i] = at[i] >= 0 ? exp2_fast((val[i] - ref) * cv) : 0.f;
-    sum += q[i];
+    for (int i = 0; i < R; ++i) {
+      q[i] = 0.f;
+      if (i * 64 >= K) continue;
+      const double each = at[i] >= 0 ? exp((double)val[i]) : 0.;
+      q[i] = (float)each;
+      in += each;
+    }
+    in = all_sum(in, lane);
+    sum = (float)in;
+    q_rest = (float)fmax(1. - in, 0.);
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      q[i] = at[i] >= 0 ? exp2_fast((val[i] - ref) * A.c) : 0.f;
+      sum += q[i];
+    }
+    sum = all_sum(sum, lane);
   }
-  sum = all_sum(sum, lane);
   const float inv = TAIL ? 1.f : 1.f / sum, ql = TAIL ? 0.f : kLn2 * log2_fast(sum);
   float log_q[R];
 #pragma unroll
@@ -409,10 +432,9 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
   const float inside = !some ? 0.f : TAIL ? sum : 1.f;
   float4 st = make_float4(m, s == 0.f ? 0.f : inside / s, m, s == 0.f ? 0.f : inside / s);
   if (TAIL && some) {
-    const float q_rest = fmaxf(1.f - sum, 0.f);
     const bool both = q_rest > 0.f && v.s > 0.f;  // (of a NaN neither is true)
     if (both) loss += q_rest * (kLn2 * (log2_fast(q_rest) + l2 - log2_fast(v.s)) - below(v.m, m, A.inv_t));
-    const float all = both ? sum + q_rest : sum;
+    const float all = both ? 1.f : sum;
     st.y = s == 0.f ? 0.f : all / s;
     st.z = v.m;
     st.w = v.s == 0.f ? 0.f : all * (rest / s) / v.s - (both ? q_rest / v.s : 0.f);
