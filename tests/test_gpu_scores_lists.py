@@ -83,3 +83,20 @@ def test_a_teacher_that_the_student_equals_has_no_divergence():
     value = torch.tensor([[0.0, 0.0, 0.0, 0.0], [math.log(3.0), 0.0, 0.0, 0.0]]).cuda()
     for tail, v in ((False, value), (True, torch.log_softmax(value, 1))):
         assert float(ops.top_distill(x, index, v, tail=tail).abs().max()) <= 40 * O.U
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("low", [-80.0, -88.0, -95.0, -103.0, -200.0, -math.inf])
+def test_repeats_of_next_to_no_probability(low, tail):
+    """A repeated class whose probabilities are subnormal or 0: it adds nothing that 32 bits show, and no infinity."""
+    from vitta_amd import ops
+    gen = torch.Generator().manual_seed(9)
+    x = torch.randn(4, 30, generator=gen)
+    index = torch.tensor([[3, 5, 5, 5], [5, 5, 3, 5], [7, 7, 7, 3], [0, 0, 0, 3]])
+    value = torch.where(index == 3, -0.25 if tail else 0.0, low)
+    leaf = x.cuda().requires_grad_()
+    loss = ops.top_distill(leaf, index.cuda(), value.cuda(), tail=tail)
+    off = (loss.detach().double().cpu() - dense_loss(x, index, value, 1.0, tail)).abs()
+    assert float(off.max()) <= bound(x, index, torch.zeros(4, 4), 1.0)
+    (grad,) = torch.autograd.grad(loss.sum(), leaf)
+    assert bool(torch.isfinite(grad).all())

@@ -415,8 +415,10 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
       }
     }
 #pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (all[i] != q[i]) log_q[i] = kLn2 * log2_fast(all[i]);
+    for (int i = 0; i < R; ++i) {
+      const bool low = all[i] < 1e-30f;  // (the logarithm takes a subnormal number for 0)
+      if (all[i] != q[i]) log_q[i] = kLn2 * (log2_fast(low ? all[i] * 0x1p64f : all[i]) - (low ? 64.f : 0.f));
+    }
   }
   float loss = 0.f;
 #pragma unroll
