@@ -19,7 +19,7 @@ class LayerShape(C.Structure):
     _fields_ = [("outer", C.c_int64), ("C", C.c_int32), ("inner", C.c_int64), ("layout", C.c_int32)]
 
 
-SCORES_MAX_TOP, SCORES_MAX_LIST = 64, 256
+SCORES_MAX_TOP, SCORES_MAX_LIST, SCORES_MAX_CLASSES = 64, 256, 1 << 24
 CONV_MAX_TAPS = 9
 
 

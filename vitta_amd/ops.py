@@ -232,6 +232,8 @@ def _score_rows(x, name, temperature):
         raise ValueError(f"{name} must hold classes in its last dimension (got shape {tuple(x.shape)})")
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"temperature must be a positive finite number (got {temperature})")
+    if x.shape[-1] > _lib.SCORES_MAX_CLASSES and x.numel():  # (before the number meets the 32 bits of the C interface)
+        raise _lib.VittaHipError(f"{name}: unsupported number of classes {x.shape[-1]} (at most {_lib.SCORES_MAX_CLASSES})")
     return _rows_of(x)
 
 
@@ -403,6 +405,8 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
         raise ValueError("nothing is asked: give labels, top, entropy or lse")
     if labels is not None:
         labels = _score_side(labels, "labels", scores[2], scores[5], (torch.int64, torch.int32))
+        if not -2 ** 63 <= ignore_index < 2 ** 63:
+            raise ValueError(f"ignore_index must be a 64-bit number (got {ignore_index})")
     how = scores, labels, int(top), entropy, lse, float(temperature), int(ignore_index)
     if not _recorded(m):
         return LabelLogprobs(*_label_logprobs(m, *how, None))
