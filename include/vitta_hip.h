@@ -874,7 +874,7 @@ int vitta_frames_cv2_resize(const uint8_t* d_frames, int32_t n_frames, int32_t i
  * Rows of class scores (logits): what they say of a label, how sure they are, and a loss against another model's answer.
  *   d_x     scores, `classes` of them in a row; row r begins at element (r / inner_rows) outer_stride + (r % inner_rows) row_stride (any
  *           strides >= 0; a matrix: inner_rows = rows), dtype one of the VITTA_SCORES_* below, element aligned; at most 2^24 classes
- *           and 2^31 - 1 rows;  z = x / temperature,  p = softmax(z)
+ *           and 2^31 - 1 rows;  z = x / temperature (1e-30 to 1e30),  p = softmax(z)
  * vitta_label_logprobs_fwd, any of the outputs may be NULL:
  *   d_logprob [rows]      z_y - lse of label y = d_labels[row]; 0 where y == ignore_index, NaN where y is no class (nothing is read)
  *   d_entropy [rows]      -sum p log p        d_lse [rows]  log sum exp z

@@ -876,7 +876,8 @@ bool bad_out(const void* p, int32_t type) { return !p || reinterpret_cast<uintpt
 
 bool bad_scores(const void* x, int32_t type, int64_t rows, int32_t classes, int64_t stride, int64_t inner, int64_t outer, float temperature) {
   if (!x || type < VITTA_SCORES_F32 || type > VITTA_SCORES_F16 || rows <= 0 || classes <= 0 || stride < 0 || inner <= 0 || outer < 0) return true;
-  if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || temperature > 3e38f) return true;
+  // 1 / T and c stay finite, and where a difference of finite scores overflows its term is 0 beyond doubt
+  if (!(temperature >= 1e-30f && temperature <= 1e30f)) return true;
   return reinterpret_cast<uintptr_t>(x) % (type == VITTA_SCORES_F32 ? 4 : 2) != 0;
 }
 
