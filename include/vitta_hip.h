@@ -887,9 +887,11 @@ int vitta_frames_cv2_resize(const uint8_t* d_frames, int32_t n_frames, int32_t i
  * vitta_top_distill_fwd: d_loss[row] = KL(teacher's list || student)
  *   d_index, d_value [rows][list]  the teacher's classes and scores; an index that is no class (-1) is padding; a row of padding only
  *           has loss 0 and gradient 0.  A class listed twice counts with the sum of its probabilities.
- *   tail == 0: q = softmax(d_value / temperature) over the list (NaN for a list of -inf only)
+ *   tail == 0: q = softmax(d_value / temperature) over the list
  *   tail != 0: d_value are log probabilities; what they leave of 1 belongs to the classes outside the list as one class (left out
  *           where the student gives these nothing)
+ *   A row of scores with NaN or +inf, a list with NaN, or of -inf only with tail == 0: loss NaN, and the gradient NaN in every class, or 0
+ *           in every class where its upstream gradient is 0.
  *   d_q [rows][list], d_stats [rows][4]  for the backward.    list <= VITTA_SCORES_MAX_LIST
  * vitta_top_distill_bwd: d_dx [rows][classes] from d_g, a float per row at stride g_stride.
  * Workspace: vitta_scores_workspace_bytes(rows, classes, dtype, top) (top = 0 for the distillation), 16-byte aligned; one call's own until

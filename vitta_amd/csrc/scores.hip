@@ -431,17 +431,18 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
   if (lane != 0) return;
   // The gradient is e_j a - q_j: (m, a) of the listed classes, and of the others, whose e_j is taken against their own maximum: their share of
   // the rest, q_rest e_j / sum e, then holds however little the student gives them.
-  const float inside = !some ? 0.f : TAIL ? sum : 1.f;
-  float4 st = make_float4(m, s == 0.f ? 0.f : inside / s, m, s == 0.f ? 0.f : inside / s);
-  if (TAIL && some) {
+  const bool lost = s != s || (TAIL ? sum != sum : !(sum > 0.f));  // no distribution on one of the sides: NaN throughout
+  const float share = s == 0.f ? 0.f : (TAIL ? sum : 1.f) / s;
+  float4 st = make_float4(m, share, m, share);
+  if (TAIL) {
     const bool both = q_rest > 0.f && v.s > 0.f;  // (of a NaN neither is true)
     if (both) loss += q_rest * (kLn2 * (log2_fast(q_rest) + l2 - log2_fast(v.s)) - below(v.m, m, A.inv_t));
     const float all = both ? 1.f : sum;
     st.y = s == 0.f ? 0.f : all / s;
     st.z = v.m;
     st.w = v.s == 0.f ? 0.f : all * (rest / s) / v.s - (both ? q_rest / v.s : 0.f);
-    if (sum != sum || s != s) loss = nan_f();
   }
+  if (lost) loss = st.y = st.w = nan_f();
   A.loss[row] = some ? loss : 0.f;
   reinterpret_cast<float4*>(A.stats)[row] = some ? st : make_float4(m, 0.f, m, 0.f);
 }
@@ -804,7 +805,7 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
     if (tid < 64) {
       for (int k = lane; k - lane < A.list; k += 64) {
         const bool valid = k < A.list;
-        collect(valid ? A.index[row * A.list + k] : 0, valid ? -g * A.q[row * A.list + k] : 0.f, valid);
+        collect(valid ? A.index[row * A.list + k] : 0, valid && g != 0.f ? -g * A.q[row * A.list + k] : 0.f, valid);
       }
     }
     at0 = g == 0.f ? 0.f : g * st.y;
@@ -812,9 +813,10 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
   } else {
     const int64_t y = A.g_logprob ? A.labels[row] : A.ignore;
     float gl = y != A.ignore ? A.g_logprob[row * A.s_logprob] : 0.f;
-    if (y != A.ignore && (y < 0 || y >= A.classes)) gl = nan_f();
-    const float gh = ENT ? A.g_entropy[row * A.s_entropy] : 0.f;
-    float all = (A.g_lse ? A.g_lse[row * A.s_lse] : 0.f) - gl;
+    if (y != A.ignore && (y < 0 || y >= A.classes) && gl != 0.f) gl = nan_f();
+    const float gh = ENT ? A.g_entropy[row * A.s_entropy] : 0.f, gs = A.g_lse ? A.g_lse[row * A.s_lse] : 0.f;
+    float all = gs - gl;
+    bool used = gl != 0.f || gs != 0.f || gh != 0.f;
     if (tid < 64) collect(y, st.y == 0.f ? 0.f : gl * A.inv_t, y != A.ignore && lane == 0);
     if (A.g_top) {  // (every wave the whole list, of at most 64: all of them need its sum)
       const bool valid = lane < A.top;
@@ -822,10 +824,11 @@ __global__ __launch_bounds__(256) void scores_grad_kernel(BwdArgs A) {
       const float g = valid ? A.g_top[row * A.top + lane] : 0.f;
       if (tid < 64) collect(j, g * A.inv_t, j >= 0);
       all -= all_sum(j >= 0 ? g : 0.f, lane);
+      used |= __ballot(g != 0.f) != 0;
     }
     a0 = is * A.inv_t * (all + (ENT ? gh * kLn2 * st.z * is : 0.f));
     a1 = ENT ? -is * A.inv_t * gh * kLn2 : 0.f;
-    if (all == 0.f && gh == 0.f) a0 = a1 = 0.f;
+    if (!used) a0 = a1 = 0.f;  // (zeros whatever the row holds; a row of NaN that is used gets NaN, also where the gradients cancel)
     at0 = a0;
   }
   if (tid == 0) many_all[group] = many;
