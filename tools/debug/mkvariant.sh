@@ -4,6 +4,7 @@
 set -e
 cd "$(dirname "$0")/../.."
 python -m vitta_amd.build > /dev/null
+CFLAGS=$(python -c 'from vitta_amd import build; print(*build.CFLAGS)')
 NAME=$1; FLAGS=$2; shift 2 || true
 FILES=${@:-conv_b3.hip}
 mkdir -p variants /tmp/variant_$NAME
@@ -15,7 +16,7 @@ for o in vitta_amd/csrc/.build/*.o; do
   [ $skip == 0 ] && OBJS="$OBJS $o"
 done
 for f in $FILES; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC $FLAGS -c vitta_amd/csrc/$f -o /tmp/variant_$NAME/${f%.hip}.o
+  /opt/rocm/bin/hipcc $CFLAGS $FLAGS -c vitta_amd/csrc/$f -o /tmp/variant_$NAME/${f%.hip}.o
   OBJS="$OBJS /tmp/variant_$NAME/${f%.hip}.o"
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $OBJS -o variants/$NAME.so

@@ -16,6 +16,11 @@ import sys
 import tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+if ROOT not in sys.path:
+    sys.path.insert(0, ROOT)
+from vitta_amd import build  # noqa: E402
+
+COMMAND = [build.HIPCC] + build.CFLAGS + ["--cuda-device-only", "-S"]  # (the code that is shipped: other flags, other registers)
 # data operand: first for buffer stores, second (behind the address) for global / flat / scratch stores
 STORE = re.compile(r"^\s*(buffer_store_dwordx[34])\s+v\[(\d+):(\d+)\]")
 GSTORE = re.compile(r"^\s*(global_store_dwordx[34]|flat_store_dwordx[34]|scratch_store_dwordx[34])\s+(?:v\[\d+:\d+\]|v\d+|off),\s*v\[(\d+):(\d+)\]")
@@ -62,6 +67,14 @@ def scan(asm, window):
     return found
 
 
+def assembly(path):
+    """The assembly of a source as the library is built from it; subprocess.CalledProcessError where it does not compile."""
+    with tempfile.TemporaryDirectory() as tmp:
+        out = os.path.join(tmp, "k.s")
+        subprocess.run(COMMAND + [path, "-o", out], check=True, capture_output=True, text=True)
+        return open(out).read()
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--window", type=int, default=2)
@@ -74,15 +87,12 @@ def main():
     files = opt.files or sorted(glob.glob(os.path.join(ROOT, "vitta_amd", "csrc", "*.hip")))
     bad = 0
     for f in files:
-        with tempfile.TemporaryDirectory() as tmp:
-            out = os.path.join(tmp, "k.s")
-            r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "--cuda-device-only", "-S", f, "-o", out],
-                               capture_output=True, text=True)
-            if r.returncode != 0:
-                print(f"{os.path.basename(f)}: did not compile\n{r.stderr[-400:]}")
-                bad += 1
-                continue
-            hits = scan(open(out).read(), opt.window)
+        try:
+            hits = scan(assembly(f), opt.window)
+        except subprocess.CalledProcessError as e:
+            print(f"{os.path.basename(f)}: did not compile\n{e.stderr[-400:]}")
+            bad += 1
+            continue
         print(f"{os.path.basename(f)}: {len(hits)} finding(s)")
         for k, st, cl, dist in hits[:20]:
             print(f"    {k[:70]}\n        {st}\n        {cl}   (+{dist})")
