@@ -12,6 +12,7 @@ def launches(monkeypatch):
     """Host tensors pass for GPU tensors, and a launch is a line (name, arguments) in the list."""
     made = []
     monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: -1 if t.is_meta else 0)
     monkeypatch.setattr(ops, "_call", lambda name, index, *args: made.append((name, args)))
     return made
 

@@ -206,17 +206,17 @@ def _row_layout(shape, strides):
 
 
 def _rows_of(x):
-    """(the scores, (shape, type, device, strides, (rows, classes, row stride, rows of a group, stride of the groups), leading shape)); copies
+    """(the scores, (shape, type, device index, strides, (rows, classes, row stride, rows of a group, stride of the groups), leading shape)); copies
     only what has no such layout."""
     shape, stride = x.shape, x.stride()
     if len(shape) == 2 and stride[1] == 1:
-        return x, (shape, x.dtype, x.device, stride, (shape[0], shape[1], stride[0], shape[0] or 1, 0), shape[:1])
+        return x, (shape, x.dtype, x.get_device(), stride, (shape[0], shape[1], stride[0], shape[0] or 1, 0), shape[:1])
     layout = _row_layout(shape, stride) if x.numel() else (0, 1, 0)
     if layout is None:
         x = x.contiguous()
         stride = x.stride()
         layout = _row_layout(shape, stride)
-    return x, (shape, x.dtype, x.device, stride, (x.numel() // shape[-1], shape[-1]) + layout, shape[:-1])
+    return x, (shape, x.dtype, x.get_device(), stride, (x.numel() // shape[-1], shape[-1]) + layout, shape[:-1])
 
 
 def _score_rows(x, name, temperature):
@@ -228,27 +228,28 @@ def _score_rows(x, name, temperature):
         raise _lib.VittaHipError(f"{name} must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
     if x.dtype not in _SCORE_TYPES:
         raise _lib.VittaHipError(f"{name} must be float32, bfloat16 or float16 (got {x.dtype})")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    classes = x.shape[-1] if x.dim() else 0
+    if classes == 0:
         raise ValueError(f"{name} must hold classes in its last dimension (got shape {tuple(x.shape)})")
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"temperature must be a positive finite number (got {temperature})")
-    if x.shape[-1] > _lib.SCORES_MAX_CLASSES and x.numel():  # (before the number meets the 32 bits of the C interface)
-        raise _lib.VittaHipError(f"{name}: unsupported number of classes {x.shape[-1]} (at most {_lib.SCORES_MAX_CLASSES})")
+    if classes > _lib.SCORES_MAX_CLASSES and x.numel():  # (before the number meets the 32 bits of the C interface)
+        raise _lib.VittaHipError(f"{name}: unsupported number of classes {classes} (at most {_lib.SCORES_MAX_CLASSES})")
     return _rows_of(x)
 
 
-def _saved(t, shape, dtype, device, name):
+def _saved(t, shape, dtype, index, name):
     """A tensor as the forward saved it, dense.  Saved-tensor hooks (torch.autograd.graph.save_on_cpu for one) may give it back in another
     layout, so a backward takes strides and addresses from what it is given, never from the forward; another type, shape or device is an error."""
-    if t.shape == shape and t.dtype is dtype and t.device == device:
+    if t.shape == shape and t.dtype is dtype and t.get_device() == index:
         return t.contiguous()
-    raise _lib.VittaHipError(f"the saved {name} came back as {t.dtype} {tuple(t.shape)} on {t.device} (saved: {dtype} {tuple(shape)} on {device})")
+    raise _lib.VittaHipError(f"the saved {name} came back as {t.dtype} {tuple(t.shape)} on {t.device} (saved: {dtype} {tuple(shape)} on cuda:{index})")
 
 
-def _saved_rows(m, shape, dtype, device):
+def _saved_rows(m, shape, dtype, index):
     """(the saved scores, their geometry) where hooks have changed their layout"""
-    if m.shape != shape or m.dtype is not dtype or m.device != device:
-        _saved(m, shape, dtype, device, "scores")
+    if m.shape != shape or m.dtype is not dtype or m.get_device() != index:
+        _saved(m, shape, dtype, index, "scores")
     m, scores = _rows_of(m)
     return m, scores[4]
 
@@ -259,10 +260,10 @@ def _recorded(m):
     return m.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0
 
 
-def _score_side(t, name, device, shape, dtypes):
+def _score_side(t, name, index, shape, dtypes):
     """A companion of the scores (labels, a teacher's list): on their device, of the given shape and one of the types, dense."""
-    if t.device != device:
-        raise _lib.VittaHipError(f"{name} must live on {device} like the scores (got {t.device})")
+    if t.get_device() != index:
+        raise _lib.VittaHipError(f"{name} must live on cuda:{index} like the scores (got {t.device})")
     if t.dtype not in dtypes:
         raise _lib.VittaHipError(f"{name} must be one of {[str(d) for d in dtypes]} (got {t.dtype})")
     if t.shape != shape:
@@ -305,7 +306,7 @@ def _row_gradient(g):
 
 
 def _label_logprobs(m, scores, labels, top, entropy, lse, temperature, ignore_index, stats):
-    _, dtype, _, _, geometry, lead = scores
+    _, dtype, device, _, geometry, lead = scores
     rows, classes = geometry[:2]
     f32 = torch.float32
     a = b = c = d = e = y = None
@@ -327,7 +328,7 @@ def _label_logprobs(m, scores, labels, top, entropy, lse, temperature, ignore_in
     if rows:
         dtype = _SCORE_TYPES[dtype]
         ws, n, tickets = _score_workspace(m, rows, classes, dtype, top)
-        _call("vitta_label_logprobs_fwd", m.get_device(), m.data_ptr(), dtype, *geometry, temperature, y, ignore_index, top, a, b, c, d, e,
+        _call("vitta_label_logprobs_fwd", device, m.data_ptr(), dtype, *geometry, temperature, y, ignore_index, top, a, b, c, d, e,
               None if stats is None else stats.data_ptr(), None if ws is None else ws.data_ptr(), n, tickets)
     return logprob, ent, lse, top_logprob, top_index
 
@@ -356,7 +357,7 @@ def _label_logprobs_grad(ctx, *upstream):
     m, labels, top_index = ctx.saved_tensors
     scores, stats, top, temperature, ignore_index, asked = ctx.how
     shape, dtype, device, strides, geometry, lead = scores
-    if not (m.stride() == strides and m.shape == shape and m.dtype is dtype and m.device == device):
+    if not (m.stride() == strides and m.shape == shape and m.dtype is dtype and m.get_device() == device):
         m, geometry = _saved_rows(m, shape, dtype, device)
     dx = m.new_empty(shape)
     if geometry[0]:
@@ -375,7 +376,7 @@ def _label_logprobs_grad(ctx, *upstream):
                     label = labels.data_ptr()
             keep.append(g)
             at[i] = g.data_ptr()
-        _call("vitta_label_logprobs_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, label, ignore_index,
+        _call("vitta_label_logprobs_bwd", device, m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, label, ignore_index,
               top, index, stats.data_ptr(), at[0], stride[0], at[1], stride[1], at[2], stride[2], at[3], dx.data_ptr())
     return dx, None
 
@@ -417,7 +418,7 @@ def label_logprobs(logits, labels=None, *, top=0, entropy=True, lse=False, tempe
 
 def _top_distill(m, scores, index, value, temperature, tail):
     """(loss, the row statistics (rows, 4) and the teacher's probabilities (rows, k) in one buffer)"""
-    _, dtype, _, _, geometry, lead = scores
+    _, dtype, device, _, geometry, lead = scores
     rows, classes = geometry[:2]
     k = index.shape[-1]
     loss = m.new_empty(lead, dtype=torch.float32)
@@ -426,7 +427,7 @@ def _top_distill(m, scores, index, value, temperature, tail):
         dtype = _SCORE_TYPES[dtype]
         ws, n, tickets = _score_workspace(m, rows, classes, dtype, 0)
         stats = side.data_ptr()
-        _call("vitta_top_distill_fwd", m.get_device(), m.data_ptr(), dtype, *geometry, temperature, index.data_ptr(), value.data_ptr(),
+        _call("vitta_top_distill_fwd", device, m.data_ptr(), dtype, *geometry, temperature, index.data_ptr(), value.data_ptr(),
               _SCORE_TYPES[value.dtype], k, tail, loss.data_ptr(), stats, stats + 16 * rows, None if ws is None else ws.data_ptr(), n, tickets)
     return loss, side
 
@@ -450,14 +451,14 @@ def _top_distill_grad(ctx, g):
     m, index = ctx.saved_tensors
     scores, side, listed, temperature = ctx.how
     shape, dtype, device, strides, geometry, _ = scores
-    if not (m.stride() == strides and m.shape == shape and m.dtype is dtype and m.device == device):
+    if not (m.stride() == strides and m.shape == shape and m.dtype is dtype and m.get_device() == device):
         m, geometry = _saved_rows(m, shape, dtype, device)
     dx = m.new_empty(shape)
     if geometry[0]:
         g, stride = _row_gradient(g)
         index = _saved(index, listed, torch.int64, device, "list")
         stats = side.data_ptr()
-        _call("vitta_top_distill_bwd", m.get_device(), m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, index.data_ptr(), listed[-1],
+        _call("vitta_top_distill_bwd", device, m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, index.data_ptr(), listed[-1],
               stats, stats + 16 * geometry[0], g.data_ptr(), stride, dx.data_ptr())
     return dx, None
 
