@@ -100,3 +100,24 @@ def test_repeats_of_next_to_no_probability(low, tail):
     assert float(off.max()) <= bound(x, index, torch.zeros(4, 4), 1.0)
     (grad,) = torch.autograd.grad(loss.sum(), leaf)
     assert bool(torch.isfinite(grad).all())
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("kind", ["one slot", "strided", "neighbours"])
+def test_lists_whose_classes_meet_when_repeats_are_looked_for(kind, tail):
+    """Classes that the multiplicative hash sends to one of its 1024 slots, and regular ones, some of them twice."""
+    from vitta_amd import ops
+    classes, k = 131072, 128
+    number = torch.arange(classes)
+    one = number[((number * 2654435769) % 2 ** 32) >> 22 == 5]
+    pick = {"one slot": one[:100], "strided": number[::1024][:100], "neighbours": number[7:107]}[kind]
+    assert len(pick) == 100
+    gen = torch.Generator().manual_seed(4)
+    index = torch.stack([torch.cat([pick, pick[:28]])[torch.randperm(k, generator=gen)] for _ in range(3)])
+    value = torch.log_softmax(torch.randn(3, k + 40, generator=gen), 1)[:, :k]
+    x = torch.randn(3, classes, generator=gen)
+    loss = ops.top_distill(x.cuda(), index.cuda(), value.cuda(), tail=tail)
+    off = (loss.double().cpu() - dense_loss(x, index, value, 1.0, tail)).abs()
+    assert float(off.max()) <= bound(x, index, value, 1.0)
+    for _ in range(3):
+        assert torch.equal(ops.top_distill(x.cuda(), index.cuda(), value.cuda(), tail=tail), loss)

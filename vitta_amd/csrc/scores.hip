@@ -322,10 +322,42 @@ __device__ void finish_readout(const FwdArgs& A, int64_t row, const T* x, Sum v,
   }
 }
 
+// Bit i: entry i * 64 + lane of a list names a class that stands earlier in it already (-1: no class).  Entries meet in kSlots words of LDS by a
+// multiplicative hash (Knuth, The Art of Computer Programming 3, 6.4); of a slot the lowest (class, entry) stays, its class is done, and the
+// others meet again: two or three rounds.  (Every entry against every other by readlanes: 2048 x 32003 bfloat16 with lists of 32 five us more.)
+constexpr int kList = VITTA_SCORES_MAX_LIST / 64;
+constexpr int kSlots = 1024;
+static_assert(VITTA_SCORES_MAX_LIST <= 256 && kMaxSegments * kTailSegment <= 1 << 24, "a class and an entry share a word");
+__device__ __forceinline__ uint32_t repeats_of(const int32_t (&at)[kList], uint32_t* slots, int lane) {
+  uint32_t open = 0, again = 0;
+#pragma unroll
+  for (int i = 0; i < kList; ++i) open |= at[i] >= 0 ? 1u << i : 0u;
+  auto slot = [&](int i) { return slots + ((uint32_t)at[i] * 2654435769u >> 22); };
+  auto key = [&](int i) { return (uint32_t)at[i] << 8 | (uint32_t)(i * 64 + lane); };
+  while (__ballot(open != 0) != 0) {
+#pragma unroll
+    for (int i = 0; i < kList; ++i)
+      if (open >> i & 1) *slot(i) = ~0u;
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < kList; ++i)
+      if (open >> i & 1) atomicMin(slot(i), key(i));
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < kList; ++i)
+      if (open >> i & 1) {
+        const uint32_t least = *slot(i);
+        if (least >> 8 == (uint32_t)at[i]) open &= ~(1u << i), again |= least != key(i) ? 1u << i : 0u;
+      }
+    wave_fence();
+  }
+  return again;
+}
+
 // v: the row's sums, without the listed classes where these are one side of a tail
 template <typename T, bool TAIL>
-__device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v, int lane) {
-  constexpr int R = VITTA_SCORES_MAX_LIST / 64;
+__device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v, uint32_t* slots, int lane) {
+  constexpr int R = kList;
   const int K = A.list;
   int32_t at[R];
   float val[R], z[R];
@@ -345,17 +377,7 @@ __device__ void finish_distill(const FwdArgs& A, int64_t row, const T* x, Sum v,
     vm = fmaxf(vm, val[i]);
   }
   some = __ballot(some) != 0;
-  uint32_t again = 0;  // bit i: at[i] stands earlier in the list already
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int n = min(64, K - i * 64);
-    for (int l = 0; l < n; ++l) {
-      const int32_t j = __builtin_amdgcn_readlane(at[i], l);
-#pragma unroll
-      for (int o = i; o < R; ++o)
-        if (o * 64 < K && at[o] == j && (o > i || lane > l)) again |= 1u << o;
-    }
-  }
+  const uint32_t again = repeats_of(at, slots, lane);
   float m = v.m, s = v.s, rest = 0.f;
   if (TAIL) {  // the listed classes' own sum, each once
 #pragma unroll
@@ -454,7 +476,7 @@ template <typename V> __device__ __forceinline__ V get(const V* p) { return __hi
 
 // NW waves merge the lists (64 keys at a time, four loads ahead), the first one the sums
 template <typename T, int MODE, bool TOP, int NW>
-__device__ void join_segments(const FwdArgs& A, int64_t row, uint64_t* lists, int lane, int wave) {
+__device__ void join_segments(const FwdArgs& A, int64_t row, uint64_t* lists, uint32_t* slots, int lane, int wave) {
   const T* x = row_of<T>(A, row);
   Best best{0, false};
   if (TOP) {
@@ -481,7 +503,7 @@ __device__ void join_segments(const FwdArgs& A, int64_t row, uint64_t* lists, in
   }
   v = wave_merge(v, A.c, lane);
   if (MODE == kReadout) finish_readout<T>(A, row, x, v, best.mine, lane);
-  else finish_distill<T, MODE == kDistillTail>(A, row, x, v, lane);
+  else finish_distill<T, MODE == kDistillTail>(A, row, x, v, slots, lane);
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------------------------
@@ -491,6 +513,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
   constexpr int N = Pack<T>::N, NT = NW * 64, G = NW == 1 ? 4 : 1;  // G groups in a workgroup
   extern __shared__ __attribute__((aligned(16))) uint32_t bits_all[];  // kDistillTail: one bit per class of the group's segment
   __shared__ uint64_t keys_all[TOP ? (NW == 1 ? G : NW) * kKeys : 1];  // the waves' candidates, later their lists
+  __shared__ uint32_t slots_all[MODE == kReadout ? 1 : G * kSlots];
   __shared__ int counts[NW], last_all;
   __shared__ Sum red[NW];
   __shared__ float bounds[NW];
@@ -720,19 +743,20 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * 64, 4) void scores_kernel(FwdA
         __syncthreads();
         last = last_all;
       }
-      if (last) join_segments<T, MODE, TOP, TOP ? NW : 1>(A, row, keys_all, lane, wave);
+      if (last) join_segments<T, MODE, TOP, TOP ? NW : 1>(A, row, keys_all, slots_all, lane, wave);
       return;
     }
   }
   if (MODE == kReadout) finish_readout<T>(A, row, whole, v, best.mine, lane);
-  else finish_distill<T, MODE == kDistillTail>(A, row, whole, v, lane);
+  else finish_distill<T, MODE == kDistillTail>(A, row, whole, v, slots_all + (NW == 1 && MODE != kReadout ? wave * kSlots : 0), lane);
 }
 
 // a launch of its own for the joins
 template <typename T, int MODE, bool TOP>
 __global__ __launch_bounds__(256) void scores_join_kernel(FwdArgs A) {
-  __shared__ uint64_t lists[4 * 64];
-  join_segments<T, MODE, TOP, 4>(A, A.row0 + blockIdx.x, lists, threadIdx.x & 63, threadIdx.x >> 6);
+  __shared__ uint64_t lists[TOP ? 4 * 64 : 1];
+  __shared__ uint32_t slots[MODE == kReadout ? 1 : kSlots];
+  join_segments<T, MODE, TOP, 4>(A, A.row0 + blockIdx.x, lists, slots, threadIdx.x & 63, threadIdx.x >> 6);
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------------------------
