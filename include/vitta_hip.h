@@ -875,7 +875,7 @@ int vitta_frames_cv2_resize(const uint8_t* d_frames, int32_t n_frames, int32_t i
  *   d_x     scores, `classes` of them in a row; row r begins at element (r / inner_rows) outer_stride + (r % inner_rows) row_stride (any
  *           strides >= 0; a matrix: inner_rows = rows), dtype one of the VITTA_SCORES_* below, element aligned; at most 2^24 classes
  *           and 2^31 - 1 rows;  z = x / temperature (1e-30 to 1e30),  p = softmax(z)
- * vitta_label_logprobs_fwd, any of the outputs may be NULL:
+ * vitta_label_logprobs_fwd, outputs that are not asked are NULL (d_logprob with d_labels; the two of the alternatives with top = 0):
  *   d_logprob [rows]      z_y - lse of label y = d_labels[row]; 0 where y == ignore_index, NaN where y is no class (nothing is read)
  *   d_entropy [rows]      -sum p log p        d_lse [rows]  log sum exp z
  *   d_top_logprob, d_top_index [rows][top]    the `top` highest scores in falling order, ties to the lowest class; index -1 (and log

@@ -5,7 +5,7 @@
 //   log p_j = (x_j - m) / T - ln2 log2 s        entropy = ln2 (log2 s - t / s)        lse = m / T + ln2 log2 s
 // The difference x - m is taken first, so the best score's term is exactly 1 and a row of the type's lowest value stays finite.
 // m starts at the lowest finite float: a row of minus infinities keeps s = 0 and is answered as a row without a distribution.
-// Sums, maxima and statistics are 32 bits wide; a gradient is rounded once, to the scores' type.
+// Sums, maxima and statistics are 32 bits wide, what a teacher's list leaves of 1 is summed in 64; a gradient is rounded once, to the scores' type.
 //
 // Forward: one pass, bound by memory (4096 x 131072 bfloat16: 170 us = 6.3 TB/s with label and entropy, 200 us with 64 alternatives, where the
 // candidates' instructions add up; 2048 x 32003 float16 with 5: 36 us).  A lane holds four 16-byte loads while the next four are on
@@ -234,8 +234,9 @@ struct Best {
     some = true;
   }
 
-  // every score of a row that the wave's lanes have, for rows of which the bound lets too many pass (scores that rise along the row, or many
-  // equal ones): those from the list's k-th on wait in `buf` and are taken by 64.  all(e, &f): the lane's e-th class, and its score
+  // every score of a row that the wave's lanes have, for rows of which the bound lets too many pass (scores that rise along the row, many
+  // equal ones, or a row too short to give each of its four waves a bound: 512 x 1200 bfloat16 with 5 alternatives 8.8 us, 512 x 1024 4.4,
+  // 512 x 2048 5.2): those from the list's k-th on wait in `buf` and are taken by 64.  all(e, &f): the lane's e-th class, and its score
   template <class All> __device__ void take_all(int n, int k, uint64_t* buf, All all, int lane) {
     int waiting = 0;
     float bound = kLowest;
@@ -324,7 +325,8 @@ __device__ void finish_readout(const FwdArgs& A, int64_t row, const T* x, Sum v,
 
 // Bit i: entry i * 64 + lane of a list names a class that stands earlier in it already (-1: no class).  Entries meet in kSlots words of LDS by a
 // multiplicative hash (Knuth, The Art of Computer Programming 3, 6.4); of a slot the lowest (class, entry) stays, its class is done, and the
-// others meet again: two or three rounds.  (Every entry against every other by readlanes: 2048 x 32003 bfloat16 with lists of 32 five us more.)
+// others meet again: two or three rounds.  (2048 x 32003 bfloat16 with lists of 32: 25.7 us forward, 24.9 without looking for repeats, 30 by every
+// entry against every other.)
 constexpr int kList = VITTA_SCORES_MAX_LIST / 64;
 constexpr int kSlots = 1024;
 static_assert(VITTA_SCORES_MAX_LIST <= 256 && kMaxSegments * kTailSegment <= 1 << 24, "a class and an entry share a word");
