@@ -43,3 +43,39 @@ def test_gradients_with_saved_tensor_hooks(classes, dtype, layout, how):
     for w, (out, u) in zip(want, outs):
         (g,) = torch.autograd.grad(out, x, u, retain_graph=True)
         assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_gradients_of_recomputed_scores(reentrant):
+    from torch.utils.checkpoint import checkpoint
+    from vitta_amd import ops
+    x = _scores("cut", 500, torch.float32).detach().requires_grad_()
+    labels = torch.randint(500, x.shape[:-1], generator=torch.Generator().manual_seed(5)).cuda()
+
+    def loss(y):
+        o = ops.label_logprobs(y[..., 1:] * 1.5, labels % 499, top=3)
+        return o.entropy - o.logprob + ops.top_distill(y[..., :499], o.top_index, o.top_logprob.detach(), tail=True)
+    (want,) = torch.autograd.grad(loss(x).sum(), x)
+    (got,) = torch.autograd.grad(checkpoint(loss, x, use_reentrant=False).sum(), x) if not reentrant else (None,)
+    if reentrant:
+        leaf = x.detach().clone().requires_grad_()
+        checkpoint(loss, leaf, use_reentrant=True).sum().backward()
+        got = leaf.grad
+    assert torch.equal(got, want)
+
+
+def test_what_a_backward_has_read_is_freed():
+    """A loss that is kept with its graph holds neither scores nor statistics after its backward."""
+    from vitta_amd import ops
+    x = torch.randn(4096, 300, device="cuda", requires_grad=True)
+    index = torch.arange(64, device="cuda").expand(4096, 64).contiguous()
+    value = torch.zeros(4096, 64, device="cuda")
+    held = []
+    for turn in range(3):
+        loss = ops.top_distill(x, index, value)
+        logprob = ops.label_logprobs(x, index[:, 0].contiguous(), entropy=False).logprob
+        torch.autograd.grad(loss.sum() - logprob.sum(), x)
+        if turn == 0:  # (after the first turn: what the allocator rounds, and the library's own first use)
+            before = torch.cuda.memory_allocated()
+        held.append((loss, logprob))
+    assert torch.cuda.memory_allocated() - before <= 2 * 2 * 4096 * 4 + 4 * 512

@@ -325,7 +325,7 @@ __device__ void finish_readout(const FwdArgs& A, int64_t row, const T* x, Sum v,
 
 // Bit i: entry i * 64 + lane of a list names a class that stands earlier in it already (-1: no class).  Entries meet in kSlots words of LDS by a
 // multiplicative hash (Knuth, The Art of Computer Programming 3, 6.4); of a slot the lowest (class, entry) stays, its class is done, and the
-// others meet again: two or three rounds.  (2048 x 32003 bfloat16 with lists of 32: 25.7 us forward, 24.9 without looking for repeats, 30 by every
+// others meet again: one to four rounds for random classes.  (2048 x 32003 bfloat16 with lists of 32: 25.7 us forward, 24.9 without looking for repeats, 30 by every
 // entry against every other.)
 constexpr int kList = VITTA_SCORES_MAX_LIST / 64;
 constexpr int kSlots = 1024;

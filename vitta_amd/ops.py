@@ -340,9 +340,8 @@ class _LabelLogprobs(torch.autograd.Function):
     def forward(ctx, m, how):
         stats = m.new_empty((how[0][4][0], 4), dtype=torch.float32)
         out = _label_logprobs(m, *how, stats)
-        ctx.save_for_backward(m, how[1], out[4])
-        # (the statistics, 16 bytes a row that only the backward knows, stay on the node, where no hook changes their layout)
-        ctx.how = how[0], stats, how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
+        ctx.save_for_backward(m, how[1], out[4], stats)
+        ctx.how = how[0], how[2], how[5], how[6], [i for i, t in enumerate(out) if t is not None]
         if how[2]:
             ctx.mark_non_differentiable(out[4])
         ctx.set_materialize_grads(False)
@@ -354,13 +353,14 @@ class _LabelLogprobs(torch.autograd.Function):
 
 
 def _label_logprobs_grad(ctx, *upstream):
-    m, labels, top_index = ctx.saved_tensors
-    scores, stats, top, temperature, ignore_index, asked = ctx.how
+    m, labels, top_index, stats = ctx.saved_tensors
+    scores, top, temperature, ignore_index, asked = ctx.how
     shape, dtype, device, strides, geometry, lead = scores
     if not (m.stride() == strides and m.shape == shape and m.dtype is dtype and m.get_device() == device):
         m, geometry = _saved_rows(m, shape, dtype, device)
     dx = m.new_empty(shape)
     if geometry[0]:
+        stats = _saved(stats, (geometry[0], 4), torch.float32, device, "statistics")
         at, stride, index, label = [None] * 4, [0] * 3, None, None
         keep = []  # (dense copies live until the launch is issued)
         for i, g in zip(asked, upstream):
@@ -438,8 +438,8 @@ class _TopDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, m, how):
         loss, side = _top_distill(m, *how)
-        ctx.save_for_backward(m, how[1])
-        ctx.how = how[0], side, how[1].shape, how[3]  # (the statistics as above)
+        ctx.save_for_backward(m, how[1], side)
+        ctx.how = how[0], how[1].shape, how[3]
         return loss
 
     @staticmethod
@@ -448,8 +448,8 @@ class _TopDistill(torch.autograd.Function):
 
 
 def _top_distill_grad(ctx, g):
-    m, index = ctx.saved_tensors
-    scores, side, listed, temperature = ctx.how
+    m, index, side = ctx.saved_tensors
+    scores, listed, temperature = ctx.how
     shape, dtype, device, strides, geometry, _ = scores
     if not (m.stride() == strides and m.shape == shape and m.dtype is dtype and m.get_device() == device):
         m, geometry = _saved_rows(m, shape, dtype, device)
@@ -457,6 +457,7 @@ def _top_distill_grad(ctx, g):
     if geometry[0]:
         g, stride = _row_gradient(g)
         index = _saved(index, listed, torch.int64, device, "list")
+        side = _saved(side, (geometry[0] * (4 + listed[-1]),), torch.float32, device, "statistics")
         stats = side.data_ptr()
         _call("vitta_top_distill_bwd", device, m.data_ptr(), _SCORE_TYPES[dtype], *geometry, temperature, index.data_ptr(), listed[-1],
               stats, stats + 16 * geometry[0], g.data_ptr(), stride, dx.data_ptr())
