@@ -44,6 +44,7 @@ def test_scores_without_a_tangent_are_read_in_a_dual_level(launches, call):  # n
         assert grad.shape == x.shape and len(launches) == 3
 
 
+@pytest.mark.filterwarnings("ignore")  # (the tracer's own, on its deprecation and on what it takes for constants)
 @pytest.mark.parametrize("grad", [False, True])
 @pytest.mark.parametrize("call", CALLS)
 def test_a_trace_is_refused(launches, call, grad):  # noqa: F811
